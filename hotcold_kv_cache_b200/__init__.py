@@ -23,6 +23,11 @@ __all__ = [
     "set_active_rotary_emb",
     "install_monkeypatch",
     "uninstall_monkeypatch",
+    "PagePlan",
+    "plan_pages",
+    "release_pages",
+    "append_pages",
+    "shared_prefix_attention",
 ]
 
 
@@ -30,6 +35,9 @@ def __getattr__(name):
     if name == "triton_evict_attention_forward":
         from .kernels import triton_evict_attention_forward
         return triton_evict_attention_forward
+    if name in ("PagePlan", "plan_pages", "release_pages", "append_pages", "shared_prefix_attention"):
+        from . import prefix
+        return getattr(prefix, name)
     if name == "KVController":
         from .controller import KVController
         return KVController

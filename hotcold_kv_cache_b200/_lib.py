@@ -83,6 +83,12 @@ SIGNATURES = {
     "hc_step_check": (c_int, [_P, c_int]),
     "hc_retrieve_decode": (c_int, [_P, _P, _I64, c_int, _P, c_size_t, _P]),
     "hc_encode_kmap": (c_int, [_P, _P, c_int, _I64, c_int, c_int]),
+    "hc_plan_pages": (c_int, [_P] * 5 + [c_int] * 6 + [_P] * 8),
+    "hc_release_pages": (c_int, [_P] * 5 + [c_int] * 4 + [_P] * 2),
+    "hc_append_pages": (c_int, [_P, _I64, _I64] * 3 + [_P] * 6 + [c_float] + [c_int] * 7 + [_P] * 2),
+    "hc_shared_prefix_attention_scratch_bytes": (c_size_t, [c_int] * 7),
+    "hc_shared_prefix_attention": (c_int, [_P, _I64, _I64] * 3 + [_P] * 9 + [c_int] * 10 +
+                                   [c_float, _P, c_size_t, _P]),
     "hc_step": (c_int, [_P, _P, _I64, _P, _P, _I64, _P, _P, _P, c_int, _P, c_int, c_int, _P]),
 }
 

@@ -412,4 +412,143 @@ int hc_splice_hits(const hc_layer* L, const int32_t* hit_ids, int k, void* strea
   return check_cuda(hc::launch_splice_hits(*L, hit_ids, k, reinterpret_cast<cudaStream_t>(stream)), "splice_hits");
 }
 
+// ---------------------------------------------------------------- a batch behind a shared prefix
+static int check_pages(int n_seq, int page_size, int max_blocks, int n_pages) {
+  if (n_seq <= 0 || n_seq > 4096) return fail(HC_ERR_UNSUPPORTED, "n_seq %d out of range (1..4096)", n_seq);
+  if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)))
+    return fail(HC_ERR_UNSUPPORTED, "page_size %d unsupported (a power of two, 16..256)", page_size);
+  if (max_blocks <= 0 || (int64_t)max_blocks * page_size > (1 << 30))
+    return fail(HC_ERR_ARG, "max_blocks %d out of range for pages of %d tokens", max_blocks, page_size);
+  if (n_pages <= 0) return fail(HC_ERR_ARG, "n_pages must be positive (got %d)", n_pages);
+  return HC_OK;
+}
+
+int hc_plan_pages(const int32_t* lens, const int32_t* new_lens, int32_t* block_table, const int32_t* free_pages,
+                  const int32_t* n_free, int n_seq, int page_size, int max_blocks, int n_pages, int n_tokens,
+                  int base_pos, int32_t* lens_out, int32_t* n_free_out, int32_t* cu_new, int64_t* slots,
+                  int32_t* seq_ids, int64_t* positions, int32_t* status, void* stream) {
+  if (int rc = check_pages(n_seq, page_size, max_blocks, n_pages)) return rc;
+  if (!lens || !new_lens || !block_table || !free_pages || !n_free || !lens_out || !n_free_out || !cu_new)
+    return fail(HC_ERR_ARG, "NULL tensor argument");
+  if (n_tokens < 0) return fail(HC_ERR_ARG, "n_tokens must not be negative (got %d)", n_tokens);
+  if (n_tokens > 0 && (!slots || !seq_ids || !positions)) return fail(HC_ERR_ARG, "NULL tensor argument");
+  hc::PagePlanArgs a{};
+  a.lens = const_cast<int32_t*>(lens);
+  a.new_lens = new_lens;
+  a.block_table = block_table;
+  a.free_pages = free_pages;
+  a.n_free = n_free;
+  a.lens_out = lens_out;
+  a.n_free_out = n_free_out;
+  a.cu_new = cu_new;
+  a.slots = slots;
+  a.seq_ids = seq_ids;
+  a.positions = positions;
+  a.status = status;
+  a.n_seq = n_seq, a.page_size = page_size, a.max_blocks = max_blocks, a.n_pages = n_pages;
+  a.n_tokens = n_tokens, a.base_pos = base_pos;
+  return check_cuda(hc::launch_plan_pages(a, reinterpret_cast<cudaStream_t>(stream)), "plan_pages");
+}
+
+int hc_release_pages(int32_t* lens, const int32_t* keep_lens, const int32_t* block_table, int32_t* free_pages,
+                     int32_t* n_free, int n_seq, int page_size, int max_blocks, int n_pages, int32_t* status,
+                     void* stream) {
+  if (int rc = check_pages(n_seq, page_size, max_blocks, n_pages)) return rc;
+  if (!lens || !keep_lens || !block_table || !free_pages || !n_free) return fail(HC_ERR_ARG, "NULL tensor argument");
+  hc::PagePlanArgs a{};
+  a.lens = lens;
+  a.new_lens = keep_lens;
+  a.block_table = const_cast<int32_t*>(block_table);
+  a.free_out = free_pages;
+  a.n_free = n_free;
+  a.n_free_out = n_free;
+  a.status = status;
+  a.n_seq = n_seq, a.page_size = page_size, a.max_blocks = max_blocks, a.n_pages = n_pages;
+  return check_cuda(hc::launch_release_pages(a, reinterpret_cast<cudaStream_t>(stream)), "release_pages");
+}
+
+static int check_heads(int Hq, int Hk, int D, int dtype) {
+  if (dtype < HC_F32 || dtype > HC_BF16) return fail(HC_ERR_ARG, "bad dtype %d", dtype);
+  if (D != 64 && D != 128) return fail(HC_ERR_UNSUPPORTED, "head_dim %d unsupported (64 or 128)", D);
+  if (Hk <= 0 || Hq <= 0 || Hq % Hk || Hk > 65535)
+    return fail(HC_ERR_ARG, "query heads %d must be a multiple of KV heads %d", Hq, Hk);
+  const int G = Hq / Hk;
+  if (G != 1 && G != 2 && G != 4 && G != 8) return fail(HC_ERR_UNSUPPORTED, "GQA group %d unsupported", G);
+  return HC_OK;
+}
+
+// Whether rows of D elements at `p` with these strides all start on 16 bytes.
+static bool rows16(const void* p, int64_t s0, int64_t s1, int dtype) {
+  const int64_t per = dtype == HC_F32 ? 4 : 8;
+  return aligned16(p) && s0 % per == 0 && s1 % per == 0;
+}
+
+int hc_append_pages(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh, const void* v,
+                    int64_t v_st, int64_t v_sh, void* q_out, const int64_t* slots, const int64_t* positions,
+                    void* k_pages, void* v_pages, const float* inv_freq, float rope_scaling, int n_tokens, int Hq, int Hk,
+                    int D, int page_size, int n_pages, int dtype, int32_t* status, void* stream) {
+  if (int rc = check_pages(1, page_size, 1, n_pages)) return rc;
+  if (int rc = check_heads(Hq, Hk, D, dtype)) return rc;
+  if (n_tokens < 0) return fail(HC_ERR_ARG, "n_tokens must not be negative (got %d)", n_tokens);
+  if (n_tokens == 0) return HC_OK;
+  if (!k || !v || !slots || !k_pages || !v_pages) return fail(HC_ERR_ARG, "NULL tensor argument");
+  if (q_out && !q) return fail(HC_ERR_ARG, "q_out without q");
+  if (inv_freq && !positions) return fail(HC_ERR_ARG, "the rotary needs positions");
+  if (!rows16(k, k_st, k_sh, dtype) || !rows16(v, v_st, v_sh, dtype) || !aligned16(k_pages) || !aligned16(v_pages) ||
+      (q_out && (!rows16(q, q_st, q_sh, dtype) || !aligned16(q_out))))
+    return fail(HC_ERR_ARG, "query/key/value rows must be 16-byte aligned");
+  hc::PageAppendArgs a{};
+  a.q = q, a.k = k, a.v = v;
+  a.q_st = q_st, a.q_sh = q_sh, a.k_st = k_st, a.k_sh = k_sh, a.v_st = v_st, a.v_sh = v_sh;
+  a.q_out = q_out, a.k_pages = k_pages, a.v_pages = v_pages;
+  a.slots = slots, a.positions = positions, a.inv_freq = inv_freq, a.status = status, a.rope_scaling = rope_scaling;
+  a.n_tokens = n_tokens, a.Hq = Hq, a.Hk = Hk, a.page_size = page_size, a.n_pages = n_pages;
+  return check_cuda(hc::launch_append_pages(a, dtype, D, reinterpret_cast<cudaStream_t>(stream)), "append_pages");
+}
+
+static int check_prefix(int T, int n_seq, int Hq, int Hk, int D, int P, int dtype) {
+  if (int rc = check_heads(Hq, Hk, D, dtype)) return rc;
+  if (n_seq <= 0 || n_seq > 4096) return fail(HC_ERR_UNSUPPORTED, "n_seq %d out of range (1..4096)", n_seq);
+  if (T < 0 || T > 65536) return fail(HC_ERR_UNSUPPORTED, "%d query tokens out of range (0..65536)", T);
+  if (P < 0 || P > (1 << 24)) return fail(HC_ERR_UNSUPPORTED, "prefix of %d tokens out of range (0..2^24)", P);
+  return HC_OK;
+}
+
+size_t hc_shared_prefix_attention_scratch_bytes(int dtype, int T, int n_seq, int Hq, int Hk, int D, int P) {
+  if (T == 0 || check_prefix(T, n_seq, Hq, Hk, D, P, dtype)) return 0;
+  return hc::prefix_scratch_bytes(dtype, T, n_seq, Hq, Hk, D, P);
+}
+
+int hc_shared_prefix_attention(const void* q, int64_t q_st, int64_t q_sh, const void* prefix_k, int64_t pk_sh,
+                               int64_t pk_st, const void* prefix_v, int64_t pv_sh, int64_t pv_st,
+                               const uint8_t* prefix_mask, const void* k_pages, const void* v_pages,
+                               const int32_t* block_table, const int32_t* lens, const int32_t* cu_new, void* out,
+                               float* lse, int32_t* status, int T, int n_seq, int Hq, int Hk, int D, int P,
+                               int page_size, int max_blocks, int n_pages, int dtype, float scale, void* scratch,
+                               size_t scratch_bytes, void* stream) {
+  if (int rc = check_prefix(T, n_seq, Hq, Hk, D, P, dtype)) return rc;
+  if (int rc = check_pages(n_seq, page_size, max_blocks, n_pages)) return rc;
+  if (T == 0) return HC_OK;
+  if (!q || !k_pages || !v_pages || !block_table || !lens || !cu_new || !out) return fail(HC_ERR_ARG, "NULL tensor argument");
+  if (P > 0 && (!prefix_k || !prefix_v)) return fail(HC_ERR_ARG, "a prefix of %d tokens without keys or values", P);
+  if (!(scale > 0.f) || scale > 1e30f) return fail(HC_ERR_ARG, "scaling must be positive and finite (got %g)", (double)scale);
+  if (!rows16(q, q_st, q_sh, dtype) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) ||
+      (P > 0 && (!rows16(prefix_k, pk_sh, pk_st, dtype) || !rows16(prefix_v, pv_sh, pv_st, dtype))))
+    return fail(HC_ERR_ARG, "query/key/value rows must be 16-byte aligned");
+  const size_t need = hc::prefix_scratch_bytes(dtype, T, n_seq, Hq, Hk, D, P);
+  if (!scratch || scratch_bytes < need) return fail(HC_ERR_SCRATCH, "scratch %zu < %zu bytes", scratch_bytes, need);
+  if (!aligned16(scratch)) return fail(HC_ERR_ARG, "scratch must be 16-byte aligned");
+  hc::PrefixArgs a{};
+  a.q = q, a.pk = prefix_k, a.pv = prefix_v;
+  a.q_st = q_st, a.q_sh = q_sh, a.pk_sh = pk_sh, a.pk_st = pk_st, a.pv_sh = pv_sh, a.pv_st = pv_st;
+  a.mask = prefix_mask, a.k_pages = k_pages, a.v_pages = v_pages;
+  a.block_table = block_table, a.lens = lens, a.cu_new = cu_new;
+  a.out = out, a.lse = lse, a.status = status;
+  a.T = T, a.n_seq = n_seq, a.Hq = Hq, a.Hk = Hk, a.P = P;
+  a.page_size = page_size, a.max_blocks = max_blocks, a.n_pages = n_pages;
+  a.scale = scale;
+  return check_cuda(hc::launch_prefix_attention(a, dtype, D, scratch, reinterpret_cast<cudaStream_t>(stream)),
+                    "shared_prefix_attention");
+}
+
 }  // extern "C"

@@ -62,6 +62,56 @@ cudaError_t launch_step(const hc_layer& L, const void* q, int64_t qss, const voi
 size_t step_smem_bytes(const hc_layer& L, int use_held);
 int step_parts(int Hk);
 
+// Pages of a batch's own tokens (hc_pages.cu). For a release, new_lens holds the lengths kept and
+// free_out is the stack that takes the pages back.
+struct PagePlanArgs {
+  int32_t* lens;
+  const int32_t* new_lens;
+  int32_t* block_table;  // (n_seq, max_blocks)
+  const int32_t* free_pages;
+  int32_t* free_out;
+  const int32_t* n_free;
+  int32_t* lens_out;
+  int32_t* n_free_out;
+  int32_t* cu_new;  // (n_seq + 1)
+  int64_t* slots;   // (n_tokens), as seq_ids and positions
+  int32_t* seq_ids;
+  int64_t* positions;
+  int32_t* status;
+  int n_seq, page_size, max_blocks, n_pages, n_tokens, base_pos;
+};
+struct PageAppendArgs {
+  const void *q, *k, *v;
+  int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;  // strides over tokens and heads, in elements
+  void* q_out;                                 // (n_tokens, Hq, D), or NULL
+  void *k_pages, *v_pages;                     // (n_pages, Hk, page_size, D)
+  const int64_t *slots, *positions;
+  const float* inv_freq;  // NULL: q and k are rotated already
+  int32_t* status;
+  float rope_scaling;
+  int n_tokens, Hq, Hk, page_size, n_pages;
+};
+cudaError_t launch_plan_pages(const PagePlanArgs& a, cudaStream_t stream);
+cudaError_t launch_release_pages(const PagePlanArgs& a, cudaStream_t stream);
+cudaError_t launch_append_pages(const PageAppendArgs& a, int dtype, int D, cudaStream_t stream);
+
+// Attention over [shared prefix | own pages] (hc_prefix.cu).
+struct PrefixArgs {
+  const void *q, *pk, *pv;
+  int64_t q_st, q_sh;                  // query strides over tokens and heads, in elements
+  int64_t pk_sh, pk_st, pv_sh, pv_st;  // prefix strides over heads and tokens
+  const uint8_t* mask;                 // (P) or NULL
+  const void *k_pages, *v_pages;       // (n_pages, Hk, page_size, D)
+  const int32_t *block_table, *lens, *cu_new;
+  void* out;   // (T, Hq, D)
+  float* lse;  // (T, Hq) or NULL
+  int32_t* status;
+  int T, n_seq, Hq, Hk, P, page_size, max_blocks, n_pages;
+  float scale;
+};
+size_t prefix_scratch_bytes(int dtype, int T, int n_seq, int Hq, int Hk, int D, int P);
+cudaError_t launch_prefix_attention(const PrefixArgs& a, int dtype, int D, void* scratch, cudaStream_t stream);
+
 // Set the message hc_last_error() returns on the calling thread.
 void set_last_error(const char* msg);
 

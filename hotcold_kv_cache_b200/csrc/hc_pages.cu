@@ -1,0 +1,290 @@
+// Paged storage of a batch's own tokens (the part of each sequence behind a shared prefix): block
+// tables and slot maps built from request lengths, their release, and the rotary append into pages.
+//
+// Tables. Sequence b holds len_b tokens in ceil(len_b / ps) pages of ps tokens, block_table[b][j] the
+// page of its tokens [j ps, (j + 1) ps). The free pages are a stack; the step's fresh pages come off
+// its top in the order of (sequence, block):
+//   need_b = ceil((len_b + new_b) / ps) - ceil(len_b / ps),   first_b = sum of need_a over a < b
+//   block_table[b][have_b + i] = free[n_free - 1 - first_b - i],  i < need_b
+//   token t of sequence b (cu_b <= t < cu_{b+1}) sits at p = len_b + t - cu_b, slot = page * ps + p % ps
+// It is bound by latency (a launch, two dependent loads, one block scan): 12 bytes a sequence and 20 a
+// token. Every CTA scans the lengths of all sequences for itself (at most 4096, 8 a thread), so the
+// tokens spread over a cluster of up to 8 CTAs without a second launch; a cluster, because lens and
+// n_free may be updated in place, which the first CTA does once all have read them.
+
+#include "hc_internal.cuh"
+
+namespace hc {
+
+constexpr int kPlanThreads = 512;
+constexpr int kPlanMaxSeq = 4096;
+constexpr int kPlanPer = kPlanMaxSeq / kPlanThreads;  // sequences per thread
+
+// The largest b with s[b] <= x in s[0..n), s[0] = 0 <= x, s ascending.
+__device__ __forceinline__ int last_not_above(const int* s, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (s[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ void cluster_sync_all() {
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+}
+
+__global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(PagePlanArgs a) {
+  __shared__ int s_cu[kPlanMaxSeq], s_first[kPlanMaxSeq];
+  __shared__ int s_scan[kPlanThreads / 32 + 1];
+  __shared__ long long s_tot[2];
+  pdl_wait();
+  const int tid = threadIdx.x, rank = blockIdx.x, nct = gridDim.x;
+  const int sh = __ffs(a.page_size) - 1, pm = a.page_size - 1;
+  const long long cap = (long long)a.max_blocks << sh;
+  if (tid < 2) s_tot[tid] = 0;
+  __syncthreads();
+  const int n_free = *a.n_free;
+  const int per = (a.n_seq + kPlanThreads - 1) / kPlanThreads;
+  int len[kPlanPer], add[kPlanPer];
+  int bits = (n_free < 0 || n_free > a.n_pages) ? HC_DEV_INDEX : 0;
+  long long nn = 0, np = 0;
+#pragma unroll
+  for (int i = 0; i < kPlanPer; ++i) {
+    const int b = tid * per + i;
+    if (i >= per || b >= a.n_seq) continue;
+    len[i] = a.lens[b];
+    add[i] = a.new_lens[b];
+    if (len[i] < 0 || add[i] < 0 || len[i] > cap) bits |= HC_DEV_INDEX;
+    else if (len[i] + (long long)add[i] > cap) bits |= HC_DEV_CAPACITY;
+    else {
+      nn += add[i];
+      np += (int)(((long long)len[i] + add[i] + pm) >> sh) - (int)(((long long)len[i] + pm) >> sh);
+    }
+  }
+  if (nn) atomicAdd(reinterpret_cast<unsigned long long*>(&s_tot[0]), (unsigned long long)nn);
+  if (np) atomicAdd(reinterpret_cast<unsigned long long*>(&s_tot[1]), (unsigned long long)np);
+  const int bad_index = __syncthreads_or(bits & HC_DEV_INDEX), bad_cap = __syncthreads_or(bits & HC_DEV_CAPACITY);
+  bits = (bad_index ? HC_DEV_INDEX : 0) | (bad_cap || s_tot[0] > a.n_tokens || s_tot[1] > n_free ? HC_DEV_CAPACITY : 0);
+  const bool ok = bits == 0;
+  const int total = ok ? (int)s_tot[0] : 0, fresh = ok ? (int)s_tot[1] : 0;
+  // exclusive scans of the new tokens and the fresh pages; both totals fit an int here
+  int dummy, cu = block_exclusive_scan(ok ? (int)nn : 0, s_scan, dummy);
+  int first = block_exclusive_scan(ok ? (int)np : 0, s_scan, dummy);
+#pragma unroll
+  for (int i = 0; i < kPlanPer; ++i) {
+    const int b = tid * per + i;
+    if (i >= per || b >= a.n_seq) continue;
+    s_cu[b] = cu;
+    s_first[b] = first;
+    if (rank == 0) a.cu_new[b] = cu;
+    if (ok) {
+      cu += add[i];
+      first += (int)(((long long)len[i] + add[i] + pm) >> sh) - (int)(((long long)len[i] + pm) >> sh);
+    }
+  }
+  if (tid == 0) {
+    if (rank == 0) a.cu_new[a.n_seq] = total;
+    if (rank == 0 && bits && a.status) atomicOr(a.status, bits);
+  }
+  __syncthreads();
+  const int step = nct * kPlanThreads;
+  for (int f = rank * kPlanThreads + tid; f < fresh; f += step) {
+    const int b = last_not_above(s_first, a.n_seq, f);
+    a.block_table[(size_t)b * a.max_blocks + ((a.lens[b] + pm) >> sh) + (f - s_first[b])] = a.free_pages[n_free - 1 - f];
+  }
+  for (int t = rank * kPlanThreads + tid; t < a.n_tokens; t += step) {
+    int64_t slot = -1, pos = -1;
+    int b = -1;
+    if (t < total) {
+      b = last_not_above(s_cu, a.n_seq, t);
+      const int len0 = a.lens[b], p = len0 + (t - s_cu[b]), j = p >> sh, have = (len0 + pm) >> sh;
+      const int page = j < have ? a.block_table[(size_t)b * a.max_blocks + j] : a.free_pages[n_free - 1 - s_first[b] - (j - have)];
+      if (page >= 0 && page < a.n_pages) slot = ((int64_t)page << sh) + (p & pm);
+      else if (a.status) atomicOr(a.status, HC_DEV_INDEX);
+      pos = (int64_t)a.base_pos + p;
+    }
+    a.slots[t] = slot;
+    a.seq_ids[t] = b;
+    a.positions[t] = pos;
+  }
+  if (nct > 1) cluster_sync_all();  // every CTA has read lens and n_free: they may be updated in place
+  else __syncthreads();
+  if (rank == 0) {
+#pragma unroll
+    for (int i = 0; i < kPlanPer; ++i) {
+      const int b = tid * per + i;
+      if (i < per && b < a.n_seq) a.lens_out[b] = ok ? len[i] + add[i] : len[i];
+    }
+    if (tid == 0) *a.n_free_out = n_free - fresh;
+  }
+}
+
+// Sequence b keeps its first keep_b tokens; the pages behind them go back on the stack in the reverse of
+// the order plan_pages_kernel takes them, so that taking a step back restores the stack as it was.
+__global__ void __launch_bounds__(kPlanThreads) release_pages_kernel(PagePlanArgs a) {
+  __shared__ int s_first[kPlanMaxSeq], s_have[kPlanMaxSeq];
+  __shared__ int s_scan[kPlanThreads / 32 + 1];
+  __shared__ unsigned long long s_tot;
+  pdl_wait();
+  const int tid = threadIdx.x;
+  const int sh = __ffs(a.page_size) - 1, pm = a.page_size - 1;
+  const long long cap = (long long)a.max_blocks << sh;
+  if (tid == 0) s_tot = 0;
+  __syncthreads();
+  const int n_free = *a.n_free;
+  const int per = (a.n_seq + kPlanThreads - 1) / kPlanThreads;
+  int n = 0, bits = (n_free < 0 || n_free > a.n_pages) ? HC_DEV_INDEX : 0;
+  int keep[kPlanPer], give[kPlanPer];
+#pragma unroll
+  for (int i = 0; i < kPlanPer; ++i) {
+    const int b = tid * per + i;
+    if (i >= per || b >= a.n_seq) continue;
+    const int len = a.lens[b];
+    keep[i] = a.new_lens[b];
+    give[i] = 0;
+    if (len < 0 || len > cap || keep[i] < 0 || keep[i] > len) bits |= HC_DEV_INDEX;
+    else give[i] = ((len + pm) >> sh) - ((keep[i] + pm) >> sh);
+    n += give[i];
+  }
+  if (n) atomicAdd(&s_tot, (unsigned long long)n);
+  const int bad = __syncthreads_or(bits);
+  bits = bad ? HC_DEV_INDEX : (s_tot > (unsigned long long)(a.n_pages - n_free) ? HC_DEV_CAPACITY : 0);
+  if (bits) {  // nothing is given back
+    if (tid == 0 && a.status) atomicOr(a.status, bits);
+    return;
+  }
+  const int total = (int)s_tot;
+  int dummy, first = block_exclusive_scan(n, s_scan, dummy);
+#pragma unroll
+  for (int i = 0; i < kPlanPer; ++i) {
+    const int b = tid * per + i;
+    if (i >= per || b >= a.n_seq) continue;
+    s_first[b] = first;
+    s_have[b] = (keep[i] + pm) >> sh;
+    first += give[i];
+    a.lens[b] = keep[i];
+  }
+  __syncthreads();
+  for (int f = tid; f < total; f += kPlanThreads) {
+    const int b = last_not_above(s_first, a.n_seq, f);
+    a.free_out[n_free + total - 1 - f] = a.block_table[(size_t)b * a.max_blocks + s_have[b] + (f - s_first[b])];
+  }
+  if (tid == 0) *a.n_free_out = n_free + total;
+}
+
+cudaError_t launch_plan_pages(const PagePlanArgs& a, cudaStream_t stream) {
+  // one CTA for what a CTA does in a few rounds, up to 8 for the slot maps of whole prompts
+  int ctas = 1;
+  while (ctas < 8 && (int64_t)ctas * kPlanThreads * 4 < a.n_tokens) ctas *= 2;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)ctas;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)ctas);
+  cfg.blockDim = dim3(kPlanThreads);
+  cfg.stream = stream;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cudaLaunchKernelEx(&cfg, plan_pages_kernel, a);
+}
+
+cudaError_t launch_release_pages(const PagePlanArgs& a, cudaStream_t stream) {
+  return launch_pdl(release_pages_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a);
+}
+
+// ----------------------------------------------------------------------------------------
+// Rotary append: x'[i] = x[i] cos - x[i + D/2] sin, x'[i + D/2] = x[i + D/2] cos + x[i] sin with the
+// angle position * inv_freq[i], for queries and keys; keys and values go to the row their slot names.
+// Bound by HBM: every element is read once and written once. A CTA takes one token; its 16-byte pairs
+// of chunks (i, i + D/2) are loaded while D/2 threads work out the token's angles.
+// The angle is reduced in 64 bits (a 32-bit product is off by 0.008 rad at position 131072) and the
+// rotation is done in 32 bits and rounded once.
+// ----------------------------------------------------------------------------------------
+constexpr int kAppThreads = 256;
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kAppThreads) append_pages_kernel(PageAppendArgs a) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  constexpr int VEC = 16 / sizeof(T), H = D / 2, CH = H / VEC;  // chunks per half row
+  __shared__ float s_cos[H], s_sin[H];
+  pdl_wait();
+  const int t = blockIdx.x, tid = threadIdx.x;
+  const int64_t slot = a.slots[t];
+  if (slot < 0 || slot >= (int64_t)a.n_pages * a.page_size) {
+    if (slot != -1 && tid == 0 && a.status) atomicOr(a.status, HC_DEV_INDEX);
+    return;
+  }
+  const int64_t page = slot / a.page_size, row = slot % a.page_size;
+  if (a.inv_freq && tid < H) {
+    const double ang = (double)a.inv_freq[tid] * (double)a.positions[t];
+    const double n = rint(ang * 0.15915494309189535);  // 1 / (2 pi)
+    // 2 pi as the nearest double and what that leaves
+    const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, ang));
+    float c, s;
+    sincosf((float)r, &s, &c);
+    s_cos[tid] = c * a.rope_scaling;
+    s_sin[tid] = s * a.rope_scaling;
+  }
+  __syncthreads();
+  const T* q = reinterpret_cast<const T*>(a.q) + t * a.q_st;
+  const T* k = reinterpret_cast<const T*>(a.k) + t * a.k_st;
+  const T* v = reinterpret_cast<const T*>(a.v) + t * a.v_st;
+  T* qo = reinterpret_cast<T*>(a.q_out) + (size_t)t * a.Hq * D;
+  const int nq = a.q_out ? a.Hq : 0;
+  const int rot = (nq + a.Hk) * CH;
+  for (int x = tid; x < rot + a.Hk * CH; x += kAppThreads) {
+    const int hh = x / CH, c = x % CH;
+    const T* src;
+    T* dst;
+    bool turn = a.inv_freq != nullptr;
+    if (hh < nq) {
+      src = q + hh * a.q_sh;
+      dst = qo + (size_t)hh * D;
+    } else if (hh < nq + a.Hk) {
+      const int h = hh - nq;
+      src = k + h * a.k_sh;
+      dst = reinterpret_cast<T*>(a.k_pages) + (((size_t)page * a.Hk + h) * a.page_size + row) * D;
+    } else {
+      const int h = hh - nq - a.Hk;
+      src = v + h * a.v_sh;
+      dst = reinterpret_cast<T*>(a.v_pages) + (((size_t)page * a.Hk + h) * a.page_size + row) * D;
+      turn = false;
+    }
+    uint4 lo = reinterpret_cast<const uint4*>(src)[c], hi = reinterpret_cast<const uint4*>(src + H)[c];
+    if (turn) {
+      float fl[VEC], fh[VEC];
+      unpack16<DT>(lo, fl);
+      unpack16<DT>(hi, fh);
+      alignas(16) T ol[VEC], oh[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) {
+        const float cs = s_cos[c * VEC + e], sn = s_sin[c * VEC + e];
+        ol[e] = E::from_f(fl[e] * cs - fh[e] * sn);
+        oh[e] = E::from_f(fh[e] * cs + fl[e] * sn);
+      }
+      lo = *reinterpret_cast<uint4*>(ol);
+      hi = *reinterpret_cast<uint4*>(oh);
+    }
+    reinterpret_cast<uint4*>(dst)[c] = lo;
+    reinterpret_cast<uint4*>(dst + H)[c] = hi;
+  }
+}
+
+template <int DT, int D>
+static cudaError_t append_pages_t(const PageAppendArgs& a, cudaStream_t stream) {
+  return launch_pdl(append_pages_kernel<DT, D>, dim3((unsigned)a.n_tokens), dim3(kAppThreads), 0, stream, a);
+}
+
+cudaError_t launch_append_pages(const PageAppendArgs& a, int dtype, int D, cudaStream_t stream) {
+  HC_DISPATCH_DT_D(dtype, D, append_pages_t, a, stream);
+}
+
+}  // namespace hc

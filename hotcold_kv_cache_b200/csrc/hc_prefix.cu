@@ -1,0 +1,389 @@
+// Attention of a batch over [shared prefix | the sequence's own pages]:
+//   o_t = sum_j softmax_j(scale q_t . k_j) v_j,  j over the unmasked prefix keys and own keys j <= len_b - n_b + i
+// (t the i-th of sequence b's n_b new tokens). The division of the work is in hc_prefix.cuh.
+//
+// prefix_simt_kernel works on 64 rows x 64 keys with fp32 FMAs; scores and probabilities pass through
+// shared memory, the output stays in registers. prefix_merge_kernel joins the partial results.
+
+#include "hc_prefix.cuh"
+
+namespace hc {
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+constexpr int kSimtThreads = 256, kSimtR = 64, kSimtK = 64;
+
+template <int D>
+struct SimtSmem {
+  static constexpr int KS = D + 4;  // padded key row: 16 rows' float4 reads hit distinct banks
+  static constexpr size_t q = 0;
+  static constexpr size_t k = q + sizeof(float) * kSimtR * D;
+  static constexpr size_t v = k + sizeof(float) * kSimtK * KS;
+  static constexpr size_t s = v + sizeof(float) * kSimtK * D;
+  static constexpr size_t al = s + sizeof(float) * kSimtR * (kSimtK + 4);
+  static constexpr size_t hd = al + sizeof(float) * kSimtR;
+  static constexpr size_t bytes = hd + sizeof(int64_t) * (kSimtThreads / 32 + 4);
+};
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kSimtThreads, 2) prefix_simt_kernel(PrefixArgs a, LineShape ls, int64_t* hdr, float2* ml,
+                                                                      float* part) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  using SM = SimtSmem<D>;
+  constexpr int VEC = 16 / sizeof(T), CPR = D / VEC, KS = SM::KS, PS = kSimtK + 4, NC = D / 64;
+  extern __shared__ __align__(16) unsigned char smem[];
+  float* sQ = reinterpret_cast<float*>(smem + SM::q);
+  float* sK = reinterpret_cast<float*>(smem + SM::k);
+  float* sV = reinterpret_cast<float*>(smem + SM::v);
+  float* sS = reinterpret_cast<float*>(smem + SM::s);
+  float* sAl = reinterpret_cast<float*>(smem + SM::al);
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, G = ls.G;
+  pdl_wait();
+  const LineGeom g(ls, min(a.T, max(a.cu_new[ls.n_seq], 0)));
+  LineWalk walk;
+  walk.c = blockIdx.x;
+  walk.st = line_setup<kSimtThreads>(a, ls, g, blockIdx.x, hdr, reinterpret_cast<int64_t*>(smem + SM::hd));
+  const int sh = __ffs(a.page_size) - 1;
+  const float sc = a.scale * kLog2e;
+  Piece p;
+  while (walk.next(a, ls, g, p)) {
+    const int rows = p.ntok * G;
+    __syncthreads();
+    for (int x = tid; x < kSimtR * CPR; x += kSimtThreads) {
+      const int r = x / CPR, c = x % CPR;
+      float f[VEC];
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) f[e] = 0.f;
+      if (r < rows) {
+        const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(p.tok0 + r / G) * a.q_st + (int64_t)(p.h * G + r % G) * a.q_sh;
+        unpack16<DT>(reinterpret_cast<const uint4*>(src)[c], f);
+      }
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) sQ[r * D + c * VEC + e] = f[e];
+    }
+    float o[4][4 * NC];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int j = 0; j < 4 * NC; ++j) o[i][j] = 0.f;
+    float m = kNegInf, l = 0.f;  // of row tid / 4, in units of log2
+    for (int kt = p.kt0; kt < p.kt1; ++kt) {
+      const int k0 = kt * kSimtK;
+      bool odd = false;  // a value that is not finite
+      __syncthreads();
+      for (int x = tid; x < kSimtK * CPR; x += kSimtThreads) {
+        const int r = x / CPR, c = x % CPR, key = k0 + r;
+        float fk[VEC], fv[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) fk[e] = fv[e] = 0.f;
+        const T *kr = nullptr, *vr = nullptr;
+        if (key < p.kend) {
+          if (p.own) {
+            const int page = a.block_table[(size_t)p.b * a.max_blocks + (key >> sh)];
+            if (page >= 0 && page < a.n_pages) {
+              const size_t off = (((size_t)page * ls.Hk + p.h) * a.page_size + (key & (a.page_size - 1))) * D;
+              kr = reinterpret_cast<const T*>(a.k_pages) + off;
+              vr = reinterpret_cast<const T*>(a.v_pages) + off;
+            } else if (a.status) {
+              atomicOr(a.status, HC_DEV_INDEX);
+            }
+          } else if (!a.mask || a.mask[key]) {
+            kr = reinterpret_cast<const T*>(a.pk) + p.h * a.pk_sh + (int64_t)key * a.pk_st;
+            vr = reinterpret_cast<const T*>(a.pv) + p.h * a.pv_sh + (int64_t)key * a.pv_st;
+          }
+        }
+        if (kr) {
+          unpack16<DT>(reinterpret_cast<const uint4*>(kr)[c], fk);
+          unpack16<DT>(reinterpret_cast<const uint4*>(vr)[c], fv);
+        }
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          sK[r * KS + c * VEC + e] = fk[e];
+          sV[r * D + c * VEC + e] = fv[e];
+          odd |= !isfinite(fv[e]);
+        }
+      }
+      // a causal tile whose hidden keys hold values that are not finite takes the careful product
+      const bool causal = p.own && k0 + kSimtK > p.c0 + 1;
+      const bool careful = __syncthreads_or(odd && causal);
+      float acc[4][4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+#pragma unroll 4
+      for (int d = 0; d < D; d += 4) {
+        float4 x[4], y[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(sQ + (ty * 4 + i) * D + d);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = *reinterpret_cast<const float4*>(sK + (tx + 16 * j) * KS + d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            acc[i][j] = fmaf(x[i].x, y[j].x, fmaf(x[i].y, y[j].y, fmaf(x[i].z, y[j].z, fmaf(x[i].w, y[j].w, acc[i][j]))));
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int key = k0 + tx + 16 * j;
+        const bool seen = key < p.kend && (p.own || !a.mask || a.mask[key]);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = ty * 4 + i;
+          const bool hid = p.own && key > p.c0 + r / G;
+          sS[r * PS + tx + 16 * j] = seen && !hid ? acc[i][j] * sc : kNegInf;
+        }
+      }
+      __syncthreads();
+      {  // four threads a row, 16 keys each
+        const int r = tid >> 2, part4 = tid & 3;
+        float* row = sS + r * PS + part4 * 4;
+        float x[16], mx = kNegInf;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[j * 4 + e] = row[j * 16 + e];
+            mx = fmaxf(mx, x[j * 4 + e]);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+        const float mn = fmaxf(m, mx), ref = mn == kNegInf ? 0.f : mn;
+        const float al = ex2(m - ref);
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const float pr = ex2(x[j * 4 + e] - ref);
+            row[j * 16 + e] = pr;
+            sum += pr;
+          }
+        sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+        sum += __shfl_xor_sync(0xffffffffu, sum, 2);
+        l = l * al + sum;
+        m = mn;
+        if (part4 == 0) sAl[r] = al;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float al = sAl[ty * 4 + i];
+#pragma unroll
+        for (int j = 0; j < 4 * NC; ++j) o[i][j] *= al;
+      }
+      if (!careful) {
+#pragma unroll 2
+        for (int k = 0; k < kSimtK; k += 4) {
+          float4 x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = *reinterpret_cast<const float4*>(sS + (ty * 4 + i) * PS + k);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk)
+#pragma unroll
+            for (int n = 0; n < NC; ++n) {
+              const float4 y = *reinterpret_cast<const float4*>(sV + (k + kk) * D + n * 64 + tx * 4);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                const float pr = kk == 0 ? x[i].x : kk == 1 ? x[i].y : kk == 2 ? x[i].z : x[i].w;
+                o[i][n * 4] = fmaf(pr, y.x, o[i][n * 4]);
+                o[i][n * 4 + 1] = fmaf(pr, y.y, o[i][n * 4 + 1]);
+                o[i][n * 4 + 2] = fmaf(pr, y.z, o[i][n * 4 + 2]);
+                o[i][n * 4 + 3] = fmaf(pr, y.w, o[i][n * 4 + 3]);
+              }
+            }
+        }
+      } else {
+        for (int k = 0; k < kSimtK; ++k)
+          for (int i = 0; i < 4; ++i) {
+            const int r = ty * 4 + i;
+            if (k0 + k > p.c0 + r / G) continue;  // hidden from this row: its value is not read
+            const float pr = sS[r * PS + k];
+            for (int n = 0; n < NC; ++n)
+              for (int e = 0; e < 4; ++e) o[i][n * 4 + e] = fmaf(pr, sV[k * D + n * 64 + tx * 4 + e], o[i][n * 4 + e]);
+          }
+      }
+    }
+    if ((tid & 3) == 0 && (tid >> 2) < rows) ml[p.row0 + (tid >> 2)] = make_float2(m, l);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = ty * 4 + i;
+      if (r < rows)
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+          *reinterpret_cast<float4*>(part + (size_t)(p.row0 + r) * D + n * 64 + tx * 4) =
+              make_float4(o[i][n * 4], o[i][n * 4 + 1], o[i][n * 4 + 2], o[i][n * 4 + 3]);
+    }
+  }
+}
+
+// ----------------------------------------------------------------------------------------
+// Joins the partial results of the G rows of (token, KV head): out = sum_p w_p O_p / sum_p w_p l_p with
+// w_p = 2^(m_p - max m). A CTA lists the pieces that cover the rows, then a warp takes a row. A row with
+// no attended key at all is 0 with a log-sum of -inf. Bound by the partial results it reads (from L2).
+// ----------------------------------------------------------------------------------------
+constexpr int kMergeThreads = 128;
+constexpr int kMaxCtas = 448;     // CTAs a call's work is divided among
+constexpr int kMergeList = 512;   // >= partial results of a row: one per CTA and one more per group of the row (17)
+
+template <int DT, int D>
+__global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(PrefixArgs a, LineShape s, const int64_t* hdr,
+                                                                     const float2* ml, const float* part) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  __shared__ int64_t list[kMergeList];
+  __shared__ int s_n, s_b;
+  const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  pdl_wait();
+  const int R = min(a.T, max(a.cu_new[s.n_seq], 0));
+  if (t >= R) return;  // rows behind the last sequence are left as they were
+  const LineGeom g(s, R);
+  const int64_t W = hdr[0];
+  if (tid == 0) s_b = -1;
+  __syncthreads();
+  for (int b = tid; b < s.n_seq; b += kMergeThreads)
+    if (a.cu_new[b] <= t && t < a.cu_new[b + 1]) s_b = b;
+  __syncthreads();
+  // the pieces (c, group) over these rows, in a fixed order: lane j < nch the prefix chunk j, lane nch the
+  // own pages; where a CTA ran two streams over the keys, both of its partial results
+  if (warp == 0) {
+    int64_t row = 0, second = 0;
+    int lo = 0, hi = -1;
+    if (lane < s.nch && g.ktp > 0) {
+      const int i = t / g.tt, tok0 = i * g.tt;
+      const int tiles = min(g.ct, g.ktp - lane * g.ct), rows = min(g.tt, R - tok0) * s.G;
+      const int64_t v0 = h * g.head + (int64_t)lane * g.nrt * (g.ct + kOver) + (int64_t)i * (tiles + kOver);
+      lo = (int)((v0 + kOver) / W), hi = (int)((v0 + kOver + tiles - 1) / W);
+      row = s.dup * (((int64_t)h * s.nch + lane) * s.T + tok0) * s.G + (t - tok0) * s.G;
+      second = s.dup == 2 && rows <= s.rt / 2 ? rows : 0;
+    } else if (lane == s.nch && s_b >= 0) {
+      const SeqLens q = seq_lens(a, s_b);
+      const int r = (t - q.cu) / g.tt, nr = ceil_div(q.n, g.tt), tok1 = min(q.n, (r + 1) * g.tt);
+      const int tiles = ceil_div(seq_keys(q, tok1), s.kt), rows = (tok1 - r * g.tt) * s.G;
+      if (tiles > 0) {
+        const int64_t v0 = hdr[1 + s_b] + ((int64_t)h * nr + r) * g.seq_group(s, q);
+        lo = (int)((v0 + kOver) / W), hi = (int)((v0 + kOver + tiles - 1) / W);
+        row = s.dup * ((int64_t)s.Hk * s.T * (s.P > 0 ? s.nch : 0) + (int64_t)q.cu * s.Hk + (int64_t)h * q.n + r * g.tt) * s.G +
+              (t - q.cu - r * g.tt) * s.G;
+        second = s.dup == 2 && rows <= s.rt / 2 ? rows : 0;
+      }
+    }
+    const int mine = (hi - lo + 1) * (second ? 2 : 1);
+    int at = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, at, o);
+      if (lane >= o) at += y;
+    }
+    if (lane == 31) s_n = at;
+    at -= mine;
+    for (int c = lo; c <= hi; ++c) {
+      if (at < kMergeList) list[at] = row + (int64_t)c * s.rt;
+      ++at;
+      if (second) {
+        if (at < kMergeList) list[at] = row + second + (int64_t)c * s.rt;
+        ++at;
+      }
+    }
+  }
+  __syncthreads();
+  const int n = min(s_n, kMergeList);
+  constexpr int PL = D / 32;
+  for (int gq = warp; gq < s.G; gq += kMergeThreads / 32) {
+    float M = kNegInf;
+    for (int x = lane; x < n; x += 32) M = fmaxf(M, __ldcg(&ml[list[x] + gq]).x);
+    M = warp_max(M);
+    const float ref = M == kNegInf ? 0.f : M;
+    float L = 0.f, o[PL];
+#pragma unroll
+    for (int e = 0; e < PL; ++e) o[e] = 0.f;
+#pragma unroll 4
+    for (int x = 0; x < n; ++x) {
+      const int64_t row = list[x] + gq;
+      const float2 z = __ldcg(&ml[row]);
+      const float w = ex2(z.x - ref);
+      L = fmaf(w, z.y, L);
+      const float* src = part + (size_t)row * D + lane * PL;
+      float f[PL];
+      if constexpr (PL == 4) {
+        const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
+        f[0] = y.x, f[1] = y.y, f[2] = y.z, f[3] = y.w;
+      } else {
+        const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
+        f[0] = y.x, f[1] = y.y;
+      }
+#pragma unroll
+      for (int e = 0; e < PL; ++e) o[e] = fmaf(w, f[e], o[e]);
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    alignas(16) T r[PL];
+#pragma unroll
+    for (int e = 0; e < PL; ++e) r[e] = E::from_f(L == 0.f ? 0.f : o[e] * inv);
+    const size_t orow = (size_t)t * a.Hq + (size_t)h * s.G + gq;
+    T* dst = reinterpret_cast<T*>(a.out) + orow * D + lane * PL;
+    if constexpr (sizeof(T) * PL == 16) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(r);
+    else if constexpr (sizeof(T) * PL == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(r);
+    else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(r);
+    if (a.lse && lane == 0) a.lse[orow] = L == 0.f ? kNegInf : (M + log2f(L)) * kLn2;
+  }
+}
+
+// ----------------------------------------------------------------------------------------
+// host
+// ----------------------------------------------------------------------------------------
+static int sm_count() {
+  static int n[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess) return 148;
+  int& x = n[dev & 63];
+  if (!x && (cudaDeviceGetAttribute(&x, cudaDevAttrMultiProcessorCount, dev) != cudaSuccess || x <= 0)) {
+    (void)cudaGetLastError();
+    return 148;
+  }
+  return x;
+}
+
+static LineShape prefix_shape(int dtype, int T, int n_seq, int Hq, int Hk, int P) {
+  return line_shape(T, n_seq, Hk, Hq / Hk, P, kSimtR, kSimtK, min(2 * sm_count(), kMaxCtas), 1);
+}
+
+static size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
+
+size_t prefix_scratch_bytes(int dtype, int T, int n_seq, int Hq, int Hk, int D, int P) {
+  const LineShape s = prefix_shape(dtype, T, n_seq, Hq, Hk, P);
+  const size_t rows = line_rows(s);
+  return up256(sizeof(int64_t) * (n_seq + 1)) + up256(rows * sizeof(float2)) + rows * D * sizeof(float);
+}
+
+template <int DT, int D>
+static cudaError_t prefix_t(const PrefixArgs& a, void* scratch, cudaStream_t stream) {
+  const LineShape s = prefix_shape(DT, a.T, a.n_seq, a.Hq, a.Hk, a.P);
+  char* p = static_cast<char*>(scratch);
+  int64_t* hdr = reinterpret_cast<int64_t*>(p);
+  p += up256(sizeof(int64_t) * (a.n_seq + 1));
+  float2* ml = reinterpret_cast<float2*>(p);
+  p += up256(line_rows(s) * sizeof(float2));
+  float* part = reinterpret_cast<float*>(p);
+  auto kern = prefix_simt_kernel<DT, D>;
+  const size_t smem = SimtSmem<D>::bytes;
+  cudaError_t e = ensure_smem(kern, smem);
+  if (e != cudaSuccess) return e;
+  e = launch_pdl(kern, dim3((unsigned)s.nc), dim3(kSimtThreads), smem, stream, a, s, hdr, ml, part);
+  if (e != cudaSuccess) return e;
+  return launch_pdl(prefix_merge_kernel<DT, D>, dim3((unsigned)a.T, (unsigned)a.Hk), dim3(kMergeThreads), 0, stream, a, s,
+                    (const int64_t*)hdr, (const float2*)ml, (const float*)part);
+}
+
+cudaError_t launch_prefix_attention(const PrefixArgs& a, int dtype, int D, void* scratch, cudaStream_t stream) {
+  HC_DISPATCH_DT_D(dtype, D, prefix_t, a, scratch, stream);
+}
+
+}  // namespace hc

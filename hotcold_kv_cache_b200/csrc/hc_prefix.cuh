@@ -1,0 +1,226 @@
+// How the attention of a batch over [shared prefix | own pages] is divided among CTAs.
+//
+// A query token t of sequence b sees every (unmasked) prefix key and its own sequence's keys up to
+// itself. The prefix part is the same for all sequences, so the rows (t, query head of a KV head's
+// group) of the whole batch are stacked into row tiles and each prefix key tile is read once per row
+// tile, not once per sequence. The own-pages part has row tiles per sequence. A group is
+//   prefix: (KV head, chunk of key tiles, row tile)      suffix: (sequence, KV head, row tile)
+// and all groups lie one behind the other on a line, each as long as its key tiles plus kOver (the
+// cost of starting one). CTA c works on the stretch [c W, (c + 1) W) of the line: whatever the lengths,
+// every CTA gets the same number of key tiles, and where a stretch ends inside a group the group's rows
+// are left as several partial results (running maximum, sum, unnormalised output), joined by the merge
+// kernel. A piece (c, group) has its partial rows at  2 * (rows of the groups before it) + c * ROWS:
+// pieces follow one another in c or in the group, and each takes at most min(2 rows, ROWS).
+// The prefix is cut into chunks (nch > 1) when there are several row tiles, so that row tiles reading
+// the same keys sit next to each other on the line and share them through L2.
+#pragma once
+#include "hc_internal.cuh"
+
+namespace hc {
+
+constexpr int kOver = 1;  // virtual key tiles for the start of a group
+
+// Host constants of one call.
+struct LineShape {
+  int T, n_seq, Hk, G, P;
+  int rt, kt;  // rows per row tile, keys per key tile
+  int nc;      // CTAs
+  int nch;     // prefix chunks
+  int dup;     // 2 where one piece may leave two partial results per row (two streams over the keys)
+};
+
+__host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
+
+inline LineShape line_shape(int T, int n_seq, int Hk, int G, int P, int rt, int kt, int nc, int dup) {
+  LineShape s{T, n_seq, Hk, G, P, rt, kt, nc, 1, dup};
+  const int nrt = ceil_div(T, rt / G), ktp = ceil_div(P, kt);
+  if (nrt > 1 && ktp > 0) {
+    const int want = nc / (nrt * Hk);
+    s.nch = want < 1 ? 1 : want > 16 ? 16 : want;
+    if (s.nch > ktp) s.nch = ktp;
+    s.nch = ceil_div(ktp, ceil_div(ktp, s.nch));  // no empty chunk
+  }
+  return s;
+}
+
+// Rows of partial results the call may leave.
+inline size_t line_rows(const LineShape& s) {
+  const size_t rows = (size_t)s.T * s.G * s.Hk;
+  return s.dup * (rows * (s.P > 0 ? s.nch : 0) + rows) + (size_t)s.nc * s.rt;
+}
+
+struct Piece {
+  bool own;         // suffix (own pages) or prefix
+  int b, h;         // sequence (suffix) and KV head
+  int tok0, ntok;   // query tokens
+  int kt0, kt1;     // key tiles
+  int kend;         // keys that exist for these tokens
+  int c0;           // suffix: token tok0 + i sees keys j < c0 + i + 1
+  int64_t row0;     // first partial row
+};
+
+// The lengths of sequence b as every kernel reads them: bounded, whatever the tables hold.
+struct SeqLens {
+  int cu, n, len;
+};
+__device__ __forceinline__ SeqLens seq_lens(const PrefixArgs& a, int b) {
+  SeqLens s;
+  const int c0 = min(max(a.cu_new[b], 0), a.T), c1 = min(max(a.cu_new[b + 1], 0), a.T);
+  s.cu = c0;
+  s.n = max(c1 - c0, 0);
+  const int64_t cap = (int64_t)a.max_blocks * a.page_size;
+  const int len = a.lens[b];
+  s.len = (int)min((int64_t)max(len, 0), cap);
+  if (len != s.len && a.status) atomicOr(a.status, HC_DEV_INDEX);
+  return s;
+}
+__device__ __forceinline__ int seq_keys(const SeqLens& s, int tok1) {  // keys seen by tokens below tok1 (of n)
+  return min(max(s.len - s.n + tok1, 0), s.len);
+}
+
+struct LineGeom {
+  int tt;             // query tokens per row tile
+  int nrt, ktp, ct;   // prefix row tiles, key tiles, key tiles per chunk
+  int64_t head;       // length of one KV head's prefix groups
+  int64_t vpre;       // length of all prefix groups
+  __device__ LineGeom(const LineShape& s, int R) {
+    tt = s.rt / s.G;
+    nrt = ceil_div(R, tt);
+    ktp = ceil_div(s.P, s.kt);
+    ct = ktp > 0 ? ceil_div(ktp, s.nch) : 0;
+    head = ktp > 0 ? (int64_t)nrt * (ktp + s.nch * kOver) : 0;
+    vpre = head * s.Hk;
+  }
+  __device__ int64_t seq_group(const LineShape& s, const SeqLens& q) const {  // one group of a sequence
+    return q.n > 0 && q.len > 0 ? ceil_div(q.len, s.kt) + kOver : 0;
+  }
+  __device__ int64_t seq_total(const LineShape& s, const SeqLens& q) const {
+    return seq_group(s, q) * s.Hk * ceil_div(q.n, tt);
+  }
+};
+
+// Header of the scratch: hdr[0] = W, hdr[1 + b] = where sequence b's groups start on the line.
+// Every CTA of NT threads calls it; CTA 0 writes the header. Returns the stretch of this CTA and the
+// sequence in which it starts (b0, at vb0) where that is behind the prefix.
+struct Stretch {
+  int64_t W, v, v_end, vb;
+  int b;
+};
+template <int NT>
+__device__ __forceinline__ Stretch line_setup(const PrefixArgs& a, const LineShape& s, const LineGeom& g, int c,
+                                              int64_t* hdr, int64_t* sh /* NT / 32 + 4 */) {
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  constexpr int NW = NT / 32;
+  const int per = ceil_div(s.n_seq, NT);
+  const int b0 = tid * per, b1 = min(b0 + per, s.n_seq);
+  int64_t mine = 0;
+  for (int b = b0; b < b1; ++b) mine += g.seq_total(s, seq_lens(a, b));
+  int64_t x = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += y;
+  }
+  if (lane == 31) sh[warp] = x;
+  __syncthreads();
+  int64_t before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    const int64_t t = sh[w];
+    if (w < warp) before += t;
+    total += t;
+  }
+  before += x - mine + g.vpre;
+  total += g.vpre;
+  Stretch r;
+  r.W = max((total + s.nc - 1) / s.nc, (int64_t)1);
+  r.v = min(c * r.W, total);
+  r.v_end = min((c + 1) * r.W, total);
+  if (c == 0 && tid == 0) hdr[0] = r.W;
+  // the sequence in which the stretch starts (or the first one, when it starts in the prefix)
+  const int64_t at = max(r.v, g.vpre);
+  if (tid == 0) {
+    sh[NW] = 0;
+    sh[NW + 1] = g.vpre;
+  }
+  __syncthreads();
+  int64_t vb = before;
+  for (int b = b0; b < b1; ++b) {
+    const int64_t n = g.seq_total(s, seq_lens(a, b));
+    if (c == 0) hdr[1 + b] = vb;
+    if (n > 0 && vb <= at && at < vb + n) {
+      sh[NW] = b;
+      sh[NW + 1] = vb;
+    }
+    vb += n;
+  }
+  __syncthreads();
+  r.b = (int)sh[NW];
+  r.vb = sh[NW + 1];
+  return r;
+}
+
+// The pieces of a CTA's stretch, one after the other. Uniform over the threads that walk it.
+struct LineWalk {
+  Stretch st;
+  int c;
+  __device__ __forceinline__ bool next(const PrefixArgs& a, const LineShape& s, const LineGeom& g, Piece& p) {
+    const int64_t cw = c * st.W;
+    while (st.v < st.v_end) {
+      if (st.v < g.vpre) {
+        const int h = (int)(st.v / g.head);
+        const int rem = (int)(st.v - h * g.head);
+        const int full = g.nrt * (g.ct + kOver);
+        const int j = min(rem / full, s.nch - 1);
+        const int tiles = min(g.ct, g.ktp - j * g.ct), len = tiles + kOver;
+        const int i = (rem - j * full) / len;
+        const int64_t v0 = h * g.head + (int64_t)j * full + (int64_t)i * len;
+        st.v = v0 + len;
+        const int lo = (int)max((int64_t)0, cw - v0 - kOver), hi = (int)min((int64_t)tiles, st.v_end - v0 - kOver);
+        if (lo >= hi) continue;
+        p.own = false;
+        p.b = 0;
+        p.h = h;
+        p.tok0 = i * g.tt;
+        p.ntok = min(g.tt, min(a.T, max(a.cu_new[s.n_seq], 0)) - p.tok0);
+        p.kt0 = j * g.ct + lo;
+        p.kt1 = j * g.ct + hi;
+        p.kend = s.P;
+        p.c0 = 0;
+        p.row0 = s.dup * (((int64_t)h * s.nch + j) * s.T + p.tok0) * s.G + (int64_t)c * s.rt;
+        return true;
+      }
+      if (st.b >= s.n_seq) return false;
+      const SeqLens q = seq_lens(a, st.b);
+      const int64_t n = g.seq_total(s, q);
+      if (st.v >= st.vb + n) {
+        st.vb += n;
+        ++st.b;
+        continue;
+      }
+      const int len = (int)g.seq_group(s, q), nr = ceil_div(q.n, g.tt);
+      const int x = (int)((st.v - st.vb) / len), h = x / nr, r = x % nr;
+      const int64_t v0 = st.vb + (int64_t)x * len;
+      st.v = v0 + len;
+      const int tok1 = min(q.n, (r + 1) * g.tt), keys = seq_keys(q, tok1);
+      const int tiles = ceil_div(keys, s.kt);
+      const int lo = (int)max((int64_t)0, cw - v0 - kOver), hi = (int)min((int64_t)tiles, st.v_end - v0 - kOver);
+      if (lo >= hi) continue;
+      p.own = true;
+      p.b = st.b;
+      p.h = h;
+      p.tok0 = q.cu + r * g.tt;
+      p.ntok = tok1 - r * g.tt;
+      p.kt0 = lo;
+      p.kt1 = hi;
+      p.kend = keys;
+      p.c0 = q.len - q.n + r * g.tt;
+      p.row0 = s.dup * ((int64_t)s.Hk * s.T * (s.P > 0 ? s.nch : 0) + (int64_t)q.cu * s.Hk + (int64_t)h * q.n + r * g.tt) *
+                   s.G + (int64_t)c * s.rt;
+      return true;
+    }
+    return false;
+  }
+};
+
+}  // namespace hc

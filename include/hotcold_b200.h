@@ -373,6 +373,71 @@ HC_API int hc_retrieve_query(const hc_layer* L, const void* q_dense, int64_t qd_
                              void* stream);
 HC_API int hc_splice_hits(const hc_layer* L, const int32_t* hit_ids, int k, void* stream);
 
+/*
+ * A batch behind one shared prefix (no counterpart in the reference, whose sequences each hold the
+ * whole prompt): the prefix's post-RoPE keys and values are stored once, and each sequence keeps its
+ * own tokens in pages of page_size tokens (a power of two, 16..256). k_pages / v_pages are
+ * (n_pages, Hk, page_size, D) in the model dtype; block_table (n_seq, max_blocks) int32 names the
+ * pages of each sequence in order; lens (n_seq) int32 counts its tokens; free_pages (n_pages) int32
+ * is a stack of n_free free pages. n_seq <= 4096. All of these are device memory. `status`, when not
+ * NULL, is an int32 into which HC_DEV_* bits are OR-ed.
+ *
+ * hc_plan_pages: block tables and slot maps of a step from its request lengths. Sequence b adds
+ * new_lens[b] >= 0 tokens: its fresh pages come off the stack in the order of (sequence, block) into
+ * block_table, lens_out = lens + new_lens, n_free_out = n_free - fresh pages, cu_new (n_seq + 1) is the
+ * running sum of new_lens, and for each of the n_tokens rows t of the step: seq_ids the sequence,
+ * slots = page * page_size + row in the page, positions = base_pos + place in the sequence; all three
+ * are -1 behind the last token. lens_out / n_free_out may be lens / n_free (the step is committed) or
+ * other buffers (it may be thrown away: the next plan writes over it). When the tokens exceed
+ * n_tokens, the fresh pages n_free or a sequence max_blocks, or a length is negative or out of range,
+ * nothing changes (lens_out = lens, no tokens, slots -1) and status gets HC_DEV_CAPACITY or HC_DEV_INDEX.
+ *
+ * hc_release_pages: sequence b keeps its first keep_lens[b] <= lens[b] tokens (0 frees it); pages
+ * behind them go back on the stack, in the reverse of the order a plan takes them, and lens =
+ * keep_lens. A keep_lens out of range or an overfull stack: nothing changes, status as above.
+ */
+HC_API int hc_plan_pages(const int32_t* lens, const int32_t* new_lens, int32_t* block_table, const int32_t* free_pages,
+                         const int32_t* n_free, int n_seq, int page_size, int max_blocks, int n_pages, int n_tokens,
+                         int base_pos, int32_t* lens_out, int32_t* n_free_out, int32_t* cu_new, int64_t* slots,
+                         int32_t* seq_ids, int64_t* positions, int32_t* status, void* stream);
+HC_API int hc_release_pages(int32_t* lens, const int32_t* keep_lens, const int32_t* block_table, int32_t* free_pages,
+                            int32_t* n_free, int n_seq, int page_size, int max_blocks, int n_pages, int32_t* status,
+                            void* stream);
+
+/*
+ * Rotary append of n_tokens tokens into pages: q (T,Hq,D), k and v (T,Hk,D) with strides over tokens
+ * and heads in elements. Queries and keys are rotated at positions[t] by angles position * inv_freq[i]
+ * (cos and sin times rope_scaling; computed in 32 bits or more and rounded once; inv_freq NULL: they
+ * are rotated already), queries into q_out (T,Hq,D) (NULL: none), keys and values into the page rows
+ * slots[t] names. Rows with slot -1 are left alone, q_out's too; another slot outside the pool also
+ * sets HC_DEV_INDEX. The slots of one call differ from one another.
+ */
+HC_API int hc_append_pages(const void* q, int64_t q_st, int64_t q_sh, const void* k, int64_t k_st, int64_t k_sh,
+                           const void* v, int64_t v_st, int64_t v_sh, void* q_out, const int64_t* slots,
+                           const int64_t* positions, void* k_pages, void* v_pages, const float* inv_freq,
+                           float rope_scaling, int n_tokens, int Hq, int Hk, int D, int page_size, int n_pages, int dtype,
+                           int32_t* status, void* stream);
+
+/*
+ * Attention of T query tokens (q (T,Hq,D), cu_new (n_seq + 1) their sequences' first rows) over
+ * [shared prefix | own pages]: token i of sequence b's n_b tokens attends every prefix key j < P with
+ * prefix_mask[j] != 0 (mask NULL: all) and own key j <= lens[b] - n_b + i (lens counts the step's
+ * tokens). Prefix keys and values are (Hk,P,D) with strides over heads and tokens. The prefix is read
+ * once for the whole batch. out (T,Hq,D) contiguous; lse (T,Hq) fp32, or NULL: the natural log of the
+ * sum of exponentials. A row that attends nothing is 0 with lse -inf; rows from cu_new[n_seq] on are
+ * left as they were. A block table entry outside the pool reads as zero keys and values, a length
+ * outside max_blocks pages is cut, and both set HC_DEV_INDEX. T <= 65536. Scratch from
+ * hc_shared_prefix_attention_scratch_bytes, used by one call at a time.
+ */
+HC_API size_t hc_shared_prefix_attention_scratch_bytes(int dtype, int T, int n_seq, int Hq, int Hk, int D, int P);
+HC_API int hc_shared_prefix_attention(const void* q, int64_t q_st, int64_t q_sh, const void* prefix_k, int64_t pk_sh,
+                                      int64_t pk_st, const void* prefix_v, int64_t pv_sh, int64_t pv_st,
+                                      const uint8_t* prefix_mask, const void* k_pages, const void* v_pages,
+                                      const int32_t* block_table, const int32_t* lens, const int32_t* cu_new, void* out,
+                                      float* lse, int32_t* status, int T, int n_seq, int Hq, int Hk, int D, int P,
+                                      int page_size, int max_blocks, int n_pages, int dtype, float scale, void* scratch,
+                                      size_t scratch_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

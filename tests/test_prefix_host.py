@@ -1,0 +1,83 @@
+"""CPU checks of the shared-prefix batch operators: refusals that reach no GPU, and the plain plan itself."""
+
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+import prefix_ref as R
+from hotcold_kv_cache_b200 import _lib
+
+
+def test_cpu_tensors_are_refused():
+    import hotcold_kv_cache_b200 as hc
+    i = torch.zeros(1, dtype=torch.int32)
+    q = torch.zeros(1, 2, 64)
+    pool = torch.zeros(1, 2, 16, 64)
+    with pytest.raises(ValueError, match="CUDA"):
+        hc.plan_pages(i, i, i[None], i, i, 16, 1)
+    with pytest.raises(ValueError, match="CUDA"):
+        hc.release_pages(i, i, i[None], i, i, 16)
+    with pytest.raises(ValueError, match="CUDA"):
+        hc.append_pages(q, q, q, i.long(), i.long(), pool, pool)
+    with pytest.raises(ValueError, match="CUDA"):
+        hc.shared_prefix_attention(q, None, None, pool, pool, i[None], i, torch.zeros(2, dtype=torch.int32), 0.1)
+
+
+def attend_args(**kw):
+    a = dict(q=4096, q_st=1024, q_sh=128, pk=4096, pk_sh=128, pk_st=1024, pv=4096, pv_sh=128, pv_st=1024, mask=None,
+             kp=4096, vp=4096, table=4096, lens=4096, cu=4096, out=4096, lse=None, status=None, T=1, n_seq=1, Hq=8, Hk=2,
+             D=128, P=16, page=16, blocks=1, pages=1, dtype=1, scale=0.1, scratch=None, nbytes=0, stream=None)
+    a.update(kw)
+    return list(a.values())
+
+
+@pytest.mark.parametrize("kw,word", [
+    (dict(D=96), b"head_dim"), (dict(Hq=7), b"multiple"), (dict(Hq=6), b"group"), (dict(dtype=5), b"dtype"),
+    (dict(n_seq=0), b"n_seq"), (dict(n_seq=5000), b"n_seq"), (dict(T=65537), b"query tokens"), (dict(T=-1), b"query tokens"),
+    (dict(P=-1), b"prefix"), (dict(page=24), b"page_size"), (dict(page=8), b"page_size"), (dict(page=512), b"page_size"),
+    (dict(blocks=0), b"max_blocks"), (dict(blocks=1 << 28), b"max_blocks"), (dict(pages=0), b"n_pages"),
+    (dict(q=None), b"NULL"), (dict(pk=None), b"prefix"), (dict(scale=0.0), b"scaling"), (dict(scale=float("nan")), b"scaling"),
+    (dict(q=4098), b"aligned"), (dict(q_st=1001), b"aligned"), (dict(pv_st=1001), b"aligned"), (dict(kp=4104), b"aligned"),
+    (dict(), b"scratch")])
+def test_attention_refusals_launch_nothing(kw, word):
+    lib = _lib.load()
+    assert lib.hc_shared_prefix_attention(*attend_args(**kw)) != 0
+    assert word in lib.hc_last_error()
+
+
+def test_plan_and_append_refusals_launch_nothing():
+    lib = _lib.load()
+    p = [4096] * 5
+    o = [4096] * 6 + [None, None]
+    for sizes, word in (((0, 16, 1, 1, 1, 0), b"n_seq"), ((4097, 16, 1, 1, 1, 0), b"n_seq"), ((1, 17, 1, 1, 1, 0), b"page_size"),
+                        ((1, 16, 1, 1, -1, 0), b"n_tokens")):
+        assert lib.hc_plan_pages(*p, *sizes, *o) != 0 and word in lib.hc_last_error()
+    assert lib.hc_plan_pages(None, *p[1:], 1, 16, 1, 1, 1, 0, *o) != 0 and b"NULL" in lib.hc_last_error()
+    assert lib.hc_release_pages(*p, 1, 20, 1, 1, None, None) != 0 and b"page_size" in lib.hc_last_error()
+
+    def append(T=1, Hq=8, D=128, page=16, inv=4096, k=4096, st=1024, q=4096):
+        return lib.hc_append_pages(q, st, 128, k, st, 128, 4096, st, 128, 4096, 4096, 4096, 4096, 4096, inv, 1.0, T, Hq, 2,
+                                   D, page, 1, 1, None, None)
+
+    assert append(T=0) == 0  # nothing to do, nothing launched
+    for kw, word in ((dict(T=-1), b"n_tokens"), (dict(D=80), b"head_dim"), (dict(page=4), b"page_size"),
+                     (dict(k=4100), b"aligned"), (dict(st=1023), b"aligned"), (dict(k=None), b"NULL"), (dict(q=None), b"q_out")):
+        assert append(**kw) != 0 and word in lib.hc_last_error()
+
+
+def test_scratch_grows_with_the_rows():
+    n = [_lib.size("hc_shared_prefix_attention_scratch_bytes", 1, T, 64, 32, 8, 128, 8192) for T in (0, 1, 64, 4096)]
+    assert n[0] == 0 and 0 < n[1] < n[2] < n[3] < 1 << 30
+    assert _lib.size("hc_shared_prefix_attention_scratch_bytes", 1, 1, 1, 6, 2, 128, 0) == 0
+
+
+def test_plain_plan():
+    table = np.full((2, 3), -1, np.int32)
+    table[0, 0] = 4
+    r = R.plan([15, 0], [2, 16], table, np.array([0, 1, 2, 3]), 4, 16, 19, 100)
+    assert r["slots"].tolist() == [79, 48] + list(range(32, 48)) + [-1]
+    assert r["positions"][:2].tolist() == [115, 116] and r["n_free"] == 2
+    assert r["table"].tolist() == [[4, 3, -1], [2, -1, -1]]
+    assert R.plan([15, 0], [2, 16], table, np.array([0]), 1, 16, 18, 0) is None

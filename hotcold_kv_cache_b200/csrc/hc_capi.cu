@@ -531,10 +531,17 @@ int hc_shared_prefix_attention(const void* q, int64_t q_st, int64_t q_sh, const 
   if (T == 0) return HC_OK;
   if (!q || !k_pages || !v_pages || !block_table || !lens || !cu_new || !out) return fail(HC_ERR_ARG, "NULL tensor argument");
   if (P > 0 && (!prefix_k || !prefix_v)) return fail(HC_ERR_ARG, "a prefix of %d tokens without keys or values", P);
+  // the stride of a dimension of one element says nothing
+  if (T == 1) q_st = D;
+  if (P == 1) pk_st = pv_st = D;
+  if (Hk == 1) pk_sh = pv_sh = (int64_t)P * D;
+  if (P > 0 && (pk_st <= 0 || pv_st <= 0 || pk_sh <= 0 || pv_sh <= 0))
+    return fail(HC_ERR_ARG, "prefix strides must be positive (an expanded prefix is not read in place)");
   if (!(scale > 0.f) || scale > 1e30f) return fail(HC_ERR_ARG, "scaling must be positive and finite (got %g)", (double)scale);
   if (!rows16(q, q_st, q_sh, dtype) || !aligned16(k_pages) || !aligned16(v_pages) || !aligned16(out) ||
       (P > 0 && (!rows16(prefix_k, pk_sh, pk_st, dtype) || !rows16(prefix_v, pv_sh, pv_st, dtype))))
     return fail(HC_ERR_ARG, "query/key/value rows must be 16-byte aligned");
+  if ((int64_t)n_pages * Hk * page_size > INT32_MAX) return fail(HC_ERR_UNSUPPORTED, "a pool of more than 2^31 rows");
   const size_t need = hc::prefix_scratch_bytes(dtype, T, n_seq, Hq, Hk, D, P);
   if (!scratch || scratch_bytes < need) return fail(HC_ERR_SCRATCH, "scratch %zu < %zu bytes", scratch_bytes, need);
   if (!aligned16(scratch)) return fail(HC_ERR_ARG, "scratch must be 16-byte aligned");

@@ -2,8 +2,9 @@
 //   o_t = sum_j softmax_j(scale q_t . k_j) v_j,  j over the unmasked prefix keys and own keys j <= len_b - n_b + i
 // (t the i-th of sequence b's n_b new tokens). The division of the work is in hc_prefix.cuh.
 //
-// prefix_simt_kernel works on 64 rows x 64 keys with fp32 FMAs; scores and probabilities pass through
-// shared memory, the output stays in registers. prefix_merge_kernel joins the partial results.
+// 16-bit types run on the tensor cores (hc_prefix_mma.cu). prefix_simt_kernel serves fp32 layers: 64 rows x
+// 64 keys with fp32 FMAs; scores and probabilities pass through shared memory, the output stays in
+// registers. prefix_merge_kernel joins the partial results of both.
 
 #include "hc_prefix.cuh"
 
@@ -31,9 +32,10 @@ struct SimtSmem {
   static constexpr size_t bytes = hd + sizeof(int64_t) * (kSimtThreads / 32 + 4);
 };
 
-template <int DT, int D>
+template <int D>
 __global__ void __launch_bounds__(kSimtThreads, 2) prefix_simt_kernel(PrefixArgs a, LineShape ls, int64_t* hdr, float2* ml,
                                                                       float* part) {
+  constexpr int DT = HC_F32;
   using E = Elem<DT>;
   using T = typename E::T;
   using SM = SimtSmem<D>;
@@ -320,8 +322,9 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(PrefixArgs 
         const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
         f[0] = y.x, f[1] = y.y;
       }
+      if (w != 0.f)  // a partial without a key may not have written its output
 #pragma unroll
-      for (int e = 0; e < PL; ++e) o[e] = fmaf(w, f[e], o[e]);
+        for (int e = 0; e < PL; ++e) o[e] = fmaf(w, f[e], o[e]);
     }
     const float inv = L == 0.f ? 0.f : 1.f / L;
     alignas(16) T r[PL];
@@ -352,7 +355,9 @@ static int sm_count() {
 }
 
 static LineShape prefix_shape(int dtype, int T, int n_seq, int Hq, int Hk, int P) {
-  return line_shape(T, n_seq, Hk, Hq / Hk, P, kSimtR, kSimtK, min(2 * sm_count(), kMaxCtas), 1);
+  const int sms = sm_count() < kMaxCtas / 2 ? sm_count() : kMaxCtas / 2;
+  if (dtype != HC_F32) return prefix_mma_shape(T, n_seq, Hk, Hq / Hk, P, sms);
+  return line_shape(T, n_seq, Hk, Hq / Hk, P, kSimtR, kSimtK, 2 * sms, 1);
 }
 
 static size_t up256(size_t n) { return (n + 255) & ~size_t(255); }
@@ -372,11 +377,15 @@ static cudaError_t prefix_t(const PrefixArgs& a, void* scratch, cudaStream_t str
   float2* ml = reinterpret_cast<float2*>(p);
   p += up256(line_rows(s) * sizeof(float2));
   float* part = reinterpret_cast<float*>(p);
-  auto kern = prefix_simt_kernel<DT, D>;
-  const size_t smem = SimtSmem<D>::bytes;
-  cudaError_t e = ensure_smem(kern, smem);
-  if (e != cudaSuccess) return e;
-  e = launch_pdl(kern, dim3((unsigned)s.nc), dim3(kSimtThreads), smem, stream, a, s, hdr, ml, part);
+  cudaError_t e;
+  if constexpr (DT == HC_F32) {
+    auto kern = prefix_simt_kernel<D>;
+    const size_t smem = SimtSmem<D>::bytes;
+    e = ensure_smem(kern, smem);
+    if (e == cudaSuccess) e = launch_pdl(kern, dim3((unsigned)s.nc), dim3(kSimtThreads), smem, stream, a, s, hdr, ml, part);
+  } else {
+    e = launch_prefix_mma(a, s, DT, D, hdr, ml, part, stream);
+  }
   if (e != cudaSuccess) return e;
   return launch_pdl(prefix_merge_kernel<DT, D>, dim3((unsigned)a.T, (unsigned)a.Hk), dim3(kMergeThreads), 0, stream, a, s,
                     (const int64_t*)hdr, (const float2*)ml, (const float*)part);

@@ -49,6 +49,11 @@ inline size_t line_rows(const LineShape& s) {
   return s.dup * (rows * (s.P > 0 ? s.nch : 0) + rows) + (size_t)s.nc * s.rt;
 }
 
+// The 16-bit kernel (hc_prefix_mma.cu) and its division of a call on `sms` SMs.
+LineShape prefix_mma_shape(int T, int n_seq, int Hk, int G, int P, int sms);
+cudaError_t launch_prefix_mma(const PrefixArgs& a, const LineShape& s, int dtype, int D, int64_t* hdr, float2* ml, float* part,
+                              cudaStream_t stream);
+
 struct Piece {
   bool own;         // suffix (own pages) or prefix
   int b, h;         // sequence (suffix) and KV head

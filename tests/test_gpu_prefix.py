@@ -269,6 +269,9 @@ CASES = [
     (32, 8, 128, 1500, 64, list(range(70)), [1] * 70),  # more than one row tile
     (8, 2, 64, 2049, 256, [255, 256, 257], [1, 2, 1]),
     (8, 8, 128, 128, 16, [10] * 5, [0, 0, 0, 0, 1]),
+    # a full row tile over many key tiles, then pages of one and of several key tiles in turn
+    (32, 8, 128, 9000, 64, [(b * 397) % 900 if b % 3 else b for b in range(64)], [1] * 64),
+    (16, 2, 64, 4100, 16, [(b * 211) % 600 if b % 4 else 0 for b in range(40)], [1 + b % 3 for b in range(40)]),
 ]
 
 

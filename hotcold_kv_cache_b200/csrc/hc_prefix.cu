@@ -49,9 +49,8 @@ __global__ void __launch_bounds__(kSimtThreads, 2) prefix_simt_kernel(PrefixArgs
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, G = ls.G;
   pdl_wait();
   const LineGeom g(ls, min(a.T, max(a.cu_new[ls.n_seq], 0)));
-  LineWalk walk;
-  walk.c = blockIdx.x;
-  walk.st = line_setup<kSimtThreads>(a, ls, g, blockIdx.x, hdr, reinterpret_cast<int64_t*>(smem + SM::hd));
+  LineWalk walk(a, ls, g, line_setup<kSimtThreads>(a, ls, g, blockIdx.x, hdr, reinterpret_cast<int64_t*>(smem + SM::hd)),
+                blockIdx.x);
   const int sh = __ffs(a.page_size) - 1;
   const float sc = a.scale * kLog2e;
   Piece p;
@@ -221,7 +220,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) prefix_simt_kernel(PrefixArgs
       if (r < rows)
 #pragma unroll
         for (int n = 0; n < NC; ++n)
-          *reinterpret_cast<float4*>(part + (size_t)(p.row0 + r) * D + n * 64 + tx * 4) =
+          *reinterpret_cast<float4*>(part + (size_t)p.row0 * D + ((size_t)(n * 16 + tx) * rows + r) * 4) =
               make_float4(o[i][n * 4], o[i][n * 4 + 1], o[i][n * 4 + 2], o[i][n * 4 + 3]);
     }
   }
@@ -229,8 +228,10 @@ __global__ void __launch_bounds__(kSimtThreads, 2) prefix_simt_kernel(PrefixArgs
 
 // ----------------------------------------------------------------------------------------
 // Joins the partial results of the G rows of (token, KV head): out = sum_p w_p O_p / sum_p w_p l_p with
-// w_p = 2^(m_p - max m). A CTA lists the pieces that cover the rows, then a warp takes a row. A row with
-// no attended key at all is 0 with a log-sum of -inf. Bound by the partial results it reads (from L2).
+// w_p = 2^(m_p - max m). A CTA lists the pieces that cover the rows, a warp per row works out the weights,
+// then a thread takes 16-byte columns of a row, neighbours the group's rows (they lie next to each other).
+// A row with no attended key at all is 0 with a log-sum of -inf. Bound by the partial results it reads
+// (from L2) and, for a decode step, by its launch and three dependent reads.
 // ----------------------------------------------------------------------------------------
 constexpr int kMergeThreads = 128;
 constexpr int kMaxCtas = 448;     // CTAs a call's work is divided among
@@ -242,7 +243,9 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(PrefixArgs 
   using E = Elem<DT>;
   using T = typename E::T;
   __shared__ int64_t list[kMergeList];
-  __shared__ int s_n, s_b;
+  __shared__ float wts[kMergeList * 8];
+  __shared__ float s_ml[16];
+  __shared__ int s_n[2], s_b, s_geo[4];
   const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   pdl_wait();
   const int R = min(a.T, max(a.cu_new[s.n_seq], 0));
@@ -254,30 +257,32 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(PrefixArgs 
   for (int b = tid; b < s.n_seq; b += kMergeThreads)
     if (a.cu_new[b] <= t && t < a.cu_new[b + 1]) s_b = b;
   __syncthreads();
-  // the pieces (c, group) over these rows, in a fixed order: lane j < nch the prefix chunk j, lane nch the
-  // own pages; where a CTA ran two streams over the keys, both of its partial results
+  // the blocks of partial rows over these rows, in a fixed order: lane j < nch the prefix chunk j, lane nch
+  // the own pages; where a CTA ran two streams over the keys, both of its blocks
   if (warp == 0) {
-    int64_t row = 0, second = 0;
-    int lo = 0, hi = -1;
+    int64_t row = 0;
+    int lo = 0, hi = -1, rows = 0, q0 = 0;
     if (lane < s.nch && g.ktp > 0) {
       const int i = t / g.tt, tok0 = i * g.tt;
-      const int tiles = min(g.ct, g.ktp - lane * g.ct), rows = min(g.tt, R - tok0) * s.G;
+      const int tiles = min(g.ct, g.ktp - lane * g.ct);
       const int64_t v0 = h * g.head + (int64_t)lane * g.nrt * (g.ct + kOver) + (int64_t)i * (tiles + kOver);
-      lo = (int)((v0 + kOver) / W), hi = (int)((v0 + kOver + tiles - 1) / W);
-      row = s.dup * (((int64_t)h * s.nch + lane) * s.T + tok0) * s.G + (t - tok0) * s.G;
-      second = s.dup == 2 && rows <= s.rt / 2 ? rows : 0;
+      rows = min(g.tt, R - tok0) * s.G, q0 = (t - tok0) * s.G;
+      lo = line_div(v0 + kOver, W), hi = line_div(v0 + kOver + tiles - 1, W);
+      row = s.dup * (((int64_t)h * s.nch + lane) * s.T + tok0) * s.G;
     } else if (lane == s.nch && s_b >= 0) {
       const SeqLens q = seq_lens(a, s_b);
       const int r = (t - q.cu) / g.tt, nr = ceil_div(q.n, g.tt), tok1 = min(q.n, (r + 1) * g.tt);
-      const int tiles = ceil_div(seq_keys(q, tok1), s.kt), rows = (tok1 - r * g.tt) * s.G;
+      const int tiles = ceil_div(seq_keys(q, tok1), s.kt);
+      rows = (tok1 - r * g.tt) * s.G, q0 = (t - q.cu - r * g.tt) * s.G;
       if (tiles > 0) {
         const int64_t v0 = hdr[1 + s_b] + ((int64_t)h * nr + r) * g.seq_group(s, q);
-        lo = (int)((v0 + kOver) / W), hi = (int)((v0 + kOver + tiles - 1) / W);
-        row = s.dup * ((int64_t)s.Hk * s.T * (s.P > 0 ? s.nch : 0) + (int64_t)q.cu * s.Hk + (int64_t)h * q.n + r * g.tt) * s.G +
-              (t - q.cu - r * g.tt) * s.G;
-        second = s.dup == 2 && rows <= s.rt / 2 ? rows : 0;
+        lo = line_div(v0 + kOver, W), hi = line_div(v0 + kOver + tiles - 1, W);
+        row = s.dup * ((int64_t)s.Hk * s.T * (s.P > 0 ? s.nch : 0) + (int64_t)q.cu * s.Hk + (int64_t)h * q.n + r * g.tt) * s.G;
       }
     }
+    // a row tile above 128 rows is two blocks; of a smaller one's two streams each has a block of its own
+    const bool halves = s.dup == 2 && rows > 128, second = s.dup == 2 && prefix_two_streams(rows);
+    const int blk = halves && q0 >= 128 ? 128 : 0, n_blk = halves ? min(128, rows - blk) : rows;
     const int mine = (hi - lo + 1) * (second ? 2 : 1);
     int at = mine;
 #pragma unroll
@@ -285,57 +290,75 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(PrefixArgs 
       const int y = __shfl_up_sync(0xffffffffu, at, o);
       if (lane >= o) at += y;
     }
-    if (lane == 31) s_n = at;
+    const int before = __shfl_up_sync(0xffffffffu, at, 1);
+    if (lane == 0) {
+      s_geo[0] = n_blk;  // rows of a prefix block, and the first of these rows in it
+      s_geo[1] = q0 - blk;
+    }
+    if (lane == s.nch) {
+      s_geo[2] = n_blk;
+      s_geo[3] = q0 - blk;
+      s_n[0] = min(before, kMergeList);  // prefix blocks, then those of the own pages
+      s_n[1] = min(at, kMergeList);
+    }
     at -= mine;
     for (int c = lo; c <= hi; ++c) {
-      if (at < kMergeList) list[at] = row + (int64_t)c * s.rt;
+      const int64_t base = row + (int64_t)c * s.rt + blk;
+      if (at < kMergeList) list[at] = base;
       ++at;
       if (second) {
-        if (at < kMergeList) list[at] = row + second + (int64_t)c * s.rt;
+        if (at < kMergeList) list[at] = base + rows;
         ++at;
       }
     }
   }
   __syncthreads();
-  const int n = min(s_n, kMergeList);
-  constexpr int PL = D / 32;
+  const int np = s_n[0], n = s_n[1];
   for (int gq = warp; gq < s.G; gq += kMergeThreads / 32) {
-    float M = kNegInf;
-    for (int x = lane; x < n; x += 32) M = fmaxf(M, __ldcg(&ml[list[x] + gq]).x);
+    float M = kNegInf, L = 0.f;
+    for (int x = lane; x < n; x += 32) M = fmaxf(M, __ldcg(&ml[list[x] + (x < np ? s_geo[1] : s_geo[3]) + gq]).x);
     M = warp_max(M);
     const float ref = M == kNegInf ? 0.f : M;
-    float L = 0.f, o[PL];
-#pragma unroll
-    for (int e = 0; e < PL; ++e) o[e] = 0.f;
-#pragma unroll 4
-    for (int x = 0; x < n; ++x) {
-      const int64_t row = list[x] + gq;
-      const float2 z = __ldcg(&ml[row]);
+    for (int x = lane; x < n; x += 32) {
+      const float2 z = __ldcg(&ml[list[x] + (x < np ? s_geo[1] : s_geo[3]) + gq]);
       const float w = ex2(z.x - ref);
+      wts[x * s.G + gq] = w;
       L = fmaf(w, z.y, L);
-      const float* src = part + (size_t)row * D + lane * PL;
-      float f[PL];
-      if constexpr (PL == 4) {
-        const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
-        f[0] = y.x, f[1] = y.y, f[2] = y.z, f[3] = y.w;
-      } else {
-        const float2 y = __ldcg(reinterpret_cast<const float2*>(src));
-        f[0] = y.x, f[1] = y.y;
-      }
-      if (w != 0.f)  // a partial without a key may not have written its output
-#pragma unroll
-        for (int e = 0; e < PL; ++e) o[e] = fmaf(w, f[e], o[e]);
     }
-    const float inv = L == 0.f ? 0.f : 1.f / L;
-    alignas(16) T r[PL];
-#pragma unroll
-    for (int e = 0; e < PL; ++e) r[e] = E::from_f(L == 0.f ? 0.f : o[e] * inv);
-    const size_t orow = (size_t)t * a.Hq + (size_t)h * s.G + gq;
-    T* dst = reinterpret_cast<T*>(a.out) + orow * D + lane * PL;
-    if constexpr (sizeof(T) * PL == 16) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(r);
-    else if constexpr (sizeof(T) * PL == 8) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(r);
-    else *reinterpret_cast<uint32_t*>(dst) = *reinterpret_cast<uint32_t*>(r);
-    if (a.lse && lane == 0) a.lse[orow] = L == 0.f ? kNegInf : (M + log2f(L)) * kLn2;
+    L = warp_sum(L);
+    if (lane == 0) {
+      s_ml[gq] = L;
+      if (a.lse) a.lse[(size_t)t * a.Hq + (size_t)h * s.G + gq] = L == 0.f ? kNegInf : (M + log2f(L)) * kLn2;
+    }
+  }
+  __syncthreads();
+  for (int k = tid; k < s.G * (D / 4); k += kMergeThreads) {
+    const int gq = k & (s.G - 1), c4 = k / s.G;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](int x, const float* src) {
+      const float w = wts[x * s.G + gq];
+      const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
+      if (w != 0.f) {  // a block without a key may not have been written
+        o.x = fmaf(w, y.x, o.x);
+        o.y = fmaf(w, y.y, o.y);
+        o.z = fmaf(w, y.z, o.z);
+        o.w = fmaf(w, y.w, o.w);
+      }
+    };
+    const size_t off_p = ((size_t)c4 * s_geo[0] + s_geo[1] + gq) * 4, off_s = ((size_t)c4 * s_geo[2] + s_geo[3] + gq) * 4;
+#pragma unroll 4
+    for (int x = 0; x < np; ++x) add(x, part + (size_t)list[x] * D + off_p);
+#pragma unroll 4
+    for (int x = np; x < n; ++x) add(x, part + (size_t)list[x] * D + off_s);
+    const float L = s_ml[gq], inv = L == 0.f ? 0.f : 1.f / L;
+    alignas(16) T r[4];
+    r[0] = E::from_f(L == 0.f ? 0.f : o.x * inv);
+    r[1] = E::from_f(L == 0.f ? 0.f : o.y * inv);
+    r[2] = E::from_f(L == 0.f ? 0.f : o.z * inv);
+    r[3] = E::from_f(L == 0.f ? 0.f : o.w * inv);
+    T* dst = reinterpret_cast<T*>(a.out) + ((size_t)t * a.Hq + (size_t)h * s.G + gq) * D + c4 * 4;
+    if constexpr (sizeof(T) == 4) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<uint4*>(r);
+    else *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(r);
   }
 }
 

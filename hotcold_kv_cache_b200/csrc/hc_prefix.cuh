@@ -54,6 +54,10 @@ LineShape prefix_mma_shape(int T, int n_seq, int Hk, int G, int P, int sms);
 cudaError_t launch_prefix_mma(const PrefixArgs& a, const LineShape& s, int dtype, int D, int64_t* hdr, float2* ml, float* part,
                               cudaStream_t stream);
 
+// Whether a row tile of `rows` rows is taken by two streams over its key tiles, each with a result of its own
+// (hc_prefix_mma.cu): above that its halves, below it whole pieces go to one stream each.
+__host__ __device__ inline bool prefix_two_streams(int rows) { return rows > 64 && rows <= 128; }
+
 struct Piece {
   bool own;         // suffix (own pages) or prefix
   int b, h;         // sequence (suffix) and KV head
@@ -83,12 +87,19 @@ __device__ __forceinline__ int seq_keys(const SeqLens& s, int tok1) {  // keys s
   return min(max(s.len - s.n + tok1, 0), s.len);
 }
 
+// Quotient of line positions: 64-bit division only where 32 bits do not hold them.
+__device__ __forceinline__ int line_div(int64_t x, int64_t y) {
+  return (x | y) >> 32 ? (int)(x / y) : (int)((uint32_t)x / (uint32_t)y);
+}
+
 struct LineGeom {
+  int R;              // query tokens of the call's sequences
   int tt;             // query tokens per row tile
   int nrt, ktp, ct;   // prefix row tiles, key tiles, key tiles per chunk
   int64_t head;       // length of one KV head's prefix groups
   int64_t vpre;       // length of all prefix groups
-  __device__ LineGeom(const LineShape& s, int R) {
+  __device__ LineGeom(const LineShape& s, int R_) {
+    R = R_;
     tt = s.rt / s.G;
     nrt = ceil_div(R, tt);
     ktp = ceil_div(s.P, s.kt);
@@ -118,8 +129,8 @@ __device__ __forceinline__ Stretch line_setup(const PrefixArgs& a, const LineSha
   constexpr int NW = NT / 32;
   const int per = ceil_div(s.n_seq, NT);
   const int b0 = tid * per, b1 = min(b0 + per, s.n_seq);
-  int64_t mine = 0;
-  for (int b = b0; b < b1; ++b) mine += g.seq_total(s, seq_lens(a, b));
+  int64_t mine = 0, last = 0;
+  for (int b = b0; b < b1; ++b) mine += last = g.seq_total(s, seq_lens(a, b));
   int64_t x = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -138,7 +149,7 @@ __device__ __forceinline__ Stretch line_setup(const PrefixArgs& a, const LineSha
   before += x - mine + g.vpre;
   total += g.vpre;
   Stretch r;
-  r.W = max((total + s.nc - 1) / s.nc, (int64_t)1);
+  r.W = max((int64_t)line_div(total + s.nc - 1, s.nc), (int64_t)1);
   r.v = min(c * r.W, total);
   r.v_end = min((c + 1) * r.W, total);
   if (c == 0 && tid == 0) hdr[0] = r.W;
@@ -151,7 +162,7 @@ __device__ __forceinline__ Stretch line_setup(const PrefixArgs& a, const LineSha
   __syncthreads();
   int64_t vb = before;
   for (int b = b0; b < b1; ++b) {
-    const int64_t n = g.seq_total(s, seq_lens(a, b));
+    const int64_t n = per == 1 ? last : g.seq_total(s, seq_lens(a, b));
     if (c == 0) hdr[1 + b] = vb;
     if (n > 0 && vb <= at && at < vb + n) {
       sh[NW] = b;
@@ -165,54 +176,85 @@ __device__ __forceinline__ Stretch line_setup(const PrefixArgs& a, const LineSha
   return r;
 }
 
-// The pieces of a CTA's stretch, one after the other. Uniform over the threads that walk it.
+// The pieces of a CTA's stretch, one after the other. Uniform over the threads that walk it. The position
+// is found once by division; from there groups follow one another by counting, and a sequence's lengths are
+// read once.
 struct LineWalk {
-  Stretch st;
-  int c;
+  int64_t v, v_end, cw;  // start of the current group, end and start of the stretch
+  int c, b, h, r, j;     // prefix: head h, chunk j, row tile r; own pages: sequence b, head h, row tile r
+  bool own;
+  SeqLens q;
+  int len, nr;           // own pages: length of a group, row tiles of the sequence
+  __device__ __forceinline__ void seq(const PrefixArgs& a, const LineShape& s, const LineGeom& g) {
+    q = seq_lens(a, b);
+    len = (int)g.seq_group(s, q);
+    nr = len > 0 ? ceil_div(q.n, g.tt) : 0;
+  }
+  __device__ __forceinline__ LineWalk(const PrefixArgs& a, const LineShape& s, const LineGeom& g, const Stretch& st, int cta) {
+    c = cta;
+    cw = st.v;
+    v_end = st.v_end;
+    b = st.b;
+    own = st.v >= g.vpre;
+    len = nr = h = r = j = 0;
+    v = st.v;
+    if (v >= v_end) return;
+    if (!own) {
+      h = line_div(v, g.head);
+      const int rem = (int)(v - h * g.head), full = g.nrt * (g.ct + kOver);
+      j = min(rem / full, s.nch - 1);
+      const int n = min(g.ct, g.ktp - j * g.ct) + kOver;
+      r = (rem - j * full) / n;
+      v = h * g.head + (int64_t)j * full + (int64_t)r * n;
+    } else {
+      seq(a, s, g);
+      if (len > 0) {
+        const int x = line_div(v - st.vb, len);
+        h = x / nr;
+        r = x % nr;
+        v = st.vb + (int64_t)x * len;
+      }
+    }
+  }
   __device__ __forceinline__ bool next(const PrefixArgs& a, const LineShape& s, const LineGeom& g, Piece& p) {
-    const int64_t cw = c * st.W;
-    while (st.v < st.v_end) {
-      if (st.v < g.vpre) {
-        const int h = (int)(st.v / g.head);
-        const int rem = (int)(st.v - h * g.head);
-        const int full = g.nrt * (g.ct + kOver);
-        const int j = min(rem / full, s.nch - 1);
-        const int tiles = min(g.ct, g.ktp - j * g.ct), len = tiles + kOver;
-        const int i = (rem - j * full) / len;
-        const int64_t v0 = h * g.head + (int64_t)j * full + (int64_t)i * len;
-        st.v = v0 + len;
-        const int lo = (int)max((int64_t)0, cw - v0 - kOver), hi = (int)min((int64_t)tiles, st.v_end - v0 - kOver);
-        if (lo >= hi) continue;
+    while (v < v_end) {
+      if (!own) {
+        const int tiles = min(g.ct, g.ktp - j * g.ct);
+        const int lo = (int)max((int64_t)0, cw - v - kOver), hi = (int)min((int64_t)tiles, v_end - v - kOver);
         p.own = false;
         p.b = 0;
         p.h = h;
-        p.tok0 = i * g.tt;
-        p.ntok = min(g.tt, min(a.T, max(a.cu_new[s.n_seq], 0)) - p.tok0);
+        p.tok0 = r * g.tt;
+        p.ntok = min(g.tt, g.R - p.tok0);
         p.kt0 = j * g.ct + lo;
         p.kt1 = j * g.ct + hi;
         p.kend = s.P;
         p.c0 = 0;
         p.row0 = s.dup * (((int64_t)h * s.nch + j) * s.T + p.tok0) * s.G + (int64_t)c * s.rt;
-        return true;
-      }
-      if (st.b >= s.n_seq) return false;
-      const SeqLens q = seq_lens(a, st.b);
-      const int64_t n = g.seq_total(s, q);
-      if (st.v >= st.vb + n) {
-        st.vb += n;
-        ++st.b;
+        v += tiles + kOver;
+        if (++r == g.nrt) {
+          r = 0;
+          if (++j == s.nch) {
+            j = 0;
+            if (++h == s.Hk) {
+              own = true;
+              b = h = 0;
+              if (v < v_end) seq(a, s, g);
+            }
+          }
+        }
+        if (lo < hi) return true;
         continue;
       }
-      const int len = (int)g.seq_group(s, q), nr = ceil_div(q.n, g.tt);
-      const int x = (int)((st.v - st.vb) / len), h = x / nr, r = x % nr;
-      const int64_t v0 = st.vb + (int64_t)x * len;
-      st.v = v0 + len;
-      const int tok1 = min(q.n, (r + 1) * g.tt), keys = seq_keys(q, tok1);
-      const int tiles = ceil_div(keys, s.kt);
-      const int lo = (int)max((int64_t)0, cw - v0 - kOver), hi = (int)min((int64_t)tiles, st.v_end - v0 - kOver);
-      if (lo >= hi) continue;
+      if (nr == 0) {  // a sequence without groups
+        if (++b >= s.n_seq) return false;
+        seq(a, s, g);
+        continue;
+      }
+      const int tok1 = min(q.n, (r + 1) * g.tt), keys = seq_keys(q, tok1), tiles = ceil_div(keys, s.kt);
+      const int lo = (int)max((int64_t)0, cw - v - kOver), hi = (int)min((int64_t)tiles, v_end - v - kOver);
       p.own = true;
-      p.b = st.b;
+      p.b = b;
       p.h = h;
       p.tok0 = q.cu + r * g.tt;
       p.ntok = tok1 - r * g.tt;
@@ -220,9 +262,18 @@ struct LineWalk {
       p.kt1 = hi;
       p.kend = keys;
       p.c0 = q.len - q.n + r * g.tt;
-      p.row0 = s.dup * ((int64_t)s.Hk * s.T * (s.P > 0 ? s.nch : 0) + (int64_t)q.cu * s.Hk + (int64_t)h * q.n + r * g.tt) *
-                   s.G + (int64_t)c * s.rt;
-      return true;
+      p.row0 = s.dup * ((int64_t)s.Hk * s.T * (s.P > 0 ? s.nch : 0) + (int64_t)q.cu * s.Hk + (int64_t)h * q.n + r * g.tt) * s.G +
+               (int64_t)c * s.rt;
+      v += len;
+      if (++r == nr) {
+        r = 0;
+        if (++h == s.Hk) {
+          h = 0;
+          if (++b >= s.n_seq) nr = 0, b = s.n_seq;
+          else if (v < v_end) seq(a, s, g);
+        }
+      }
+      if (lo < hi) return true;
     }
     return false;
   }

@@ -1,19 +1,23 @@
 // Attention over [shared prefix | own pages] for 16-bit types on the 5th-generation tensor cores.
 //
 // One persistent CTA per SM walks its stretch of the line (hc_prefix.cuh) in row tiles of up to 256 rows
-// and key tiles of 128. Per key tile: S = Q K^T (M = 128 rows, N = 128 keys, fp32 in TMEM), P = 2^(S scale
-// log2 e - m) rounded to the operand type (off by half a step of each probability, as large as the
-// rounding of the result itself) and written over S in TMEM, O += P V with P as the TMEM operand and V read
-// in place as an MN-major operand; O stays in TMEM for the whole piece. The softmax is online, and O is
-// only rescaled when a row's maximum has grown by more than 2^8 since the last time: until then P exceeds 1
-// by at most that, which neither type minds, and the 32-bit sums carry the same factor.
+// and key tiles of 128. Softmax is online over the key tiles: P = 2^(S scale log2 e - m), rounded to the
+// operand type (off by half a step of each probability, as large as the rounding of the result itself); O
+// stays in TMEM for the whole piece and is only rescaled when a row's maximum has grown by more than 2^8
+// since the last time: until then P exceeds 1 by at most that, which neither type minds, and the 32-bit sums
+// carry the same factor.
 //
 // Roles: warp 0 brings K and V tiles by TMA into a ring (pages as boxes of their own, absent pages as
 // boxes out of range, which read as zeros); warps 1 and 2 each issue the MMAs of one stream; warps 4-7 and
-// 8-11 are the softmax of the two streams, a thread per row. Of a row tile above 128 rows the streams take
-// a half each and share the K/V tiles; of a smaller one (a decode step of one sequence's pages, a small
-// batch) they take every second key tile of the same rows, with results of their own that the merge joins,
-// so that one stream's softmax runs under the other's MMAs in both cases.
+// 8-11 are the softmax of the two streams. What a stream is depends on the piece's rows:
+//   above 128  a half of the rows each, both over all key tiles. S = Q K^T (M = 128 rows, N = 128 keys), a
+//              thread per row; P goes back to TMEM over S as the A operand of O += P V, V read in place as
+//              an MN-major operand.
+//   65 to 128  the same rows, every second key tile each, each with a result of its own for the merge.
+//   up to 64   whole pieces in turn, transposed: S^T = K Q^T (M = 128 keys, N = the rows), a thread per key,
+//              so that all 128 threads have work where a thread per row would leave one warp 128 columns;
+//              P^T through shared memory as the B operand of O^T += V^T P^T.
+// Either way one stream's softmax runs under the other's MMAs and copies.
 //
 // Bound: HBM while 2 (rows) D flops a key cost less than its 2 D elements, i.e. up to about 256 rows a row
 // tile; beyond that the MMAs (1024 cycles per 128 x 128 x 128 pair) and the 128 x 128 exponentials (1024
@@ -27,19 +31,24 @@
 namespace hc {
 
 constexpr int kMmaThreads = 384, kMmaR = 256, kMmaK = 128;
+constexpr int kPieces = 8;    // pieces listed ahead
 constexpr float kLazy = 8.f;  // log2 of how far P may exceed 1 before O is rescaled
 
 template <int D>
 struct MmaSmem {
-  static constexpr int PL = D / 64;                 // planes of 64 elements (128 bytes, the swizzle width)
+  static constexpr int PL = D / 64;                   // planes of 64 elements (128 bytes, the swizzle width)
   static constexpr uint32_t tile = 128u * 128u * PL;  // 128 rows
-  static constexpr int NB = D == 128 ? 5 : 8;       // K/V tiles in the ring
-  static constexpr uint32_t q = 0;
-  static constexpr uint32_t ring = 2 * tile;
-  static constexpr uint32_t bars = ring + NB * tile;  // full[NB] empty[NB] s_full[2] p_ready[2] pv_done[2] q_ready[2] fin
-  static constexpr uint32_t misc = bars + 8 * (2 * NB + 9);  // tmem address, dead flag, poison[2], armed
-  static constexpr uint32_t scan = (misc + 32 + 15) & ~15u;
-  static constexpr uint32_t bytes = scan + 8 * (kMmaThreads / 32 + 4);
+  static constexpr int NB = D == 128 ? 5 : 8;         // K/V tiles in the ring
+  static constexpr uint32_t qbuf = 32768;             // per stream: Q (transposed pieces: Q, then P^T from ptr on)
+  static constexpr uint32_t pt = 16384;
+  static constexpr uint32_t ring = 2 * qbuf;
+  static constexpr uint32_t bars = ring + NB * tile;  // full[NB] empty[NB] s_full[2] p_ready[2] pv_done[2] q_ready[2] fin both
+  static constexpr uint32_t misc = (bars + 8 * (2 * NB + 10) + 15) & ~15u;  // tmem address, dead, armed, -, poison[3], turns[2]
+  static constexpr uint32_t red = misc + 48;  // per stream [4 warps][64 rows]; the setup's scan before that
+  static constexpr uint32_t pieces = red + 2 * 4 * 64 * 4;           // the next pieces, and their barriers
+  static constexpr uint32_t pbars = pieces + kPieces * sizeof(Piece);  // full[kPieces] empty[kPieces]
+  static constexpr uint32_t bytes = pbars + 16 * kPieces;
+  static_assert(bytes <= 227 * 1024, "shared memory of a CTA");
 };
 
 struct PrefixMaps {
@@ -135,6 +144,444 @@ __device__ __forceinline__ void wait_full(uint64_t* full, uint32_t n, volatile u
   wait_bar(&full[n % NB], (n / NB) & 1, dead, status);
 }
 
+// 32 lanes x N columns (N = 8, 16, 32 or 64) and back.
+template <int N>
+__device__ __forceinline__ void tmem_ld_n(uint32_t taddr, float* v) {
+  if constexpr (N == 8) {
+    tmem_ld_x8(taddr, v);
+  } else if constexpr (N == 16) {
+    tmem_ld_x8(taddr, v);
+    tmem_ld_x8(taddr + 8, v + 8);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; j += 32) tmem_ld_x32(taddr + j, v + j);
+    tmem_wait_ld();
+  }
+}
+__device__ __forceinline__ void tmem_st_x8(uint32_t taddr, const float* v) {
+  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+__device__ __forceinline__ float redux_max(float x) {
+  float y;
+  asm("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Stream x's turn for its tall tile number n: the first stream goes when the other has issued all S tiles
+// before n, the second when the first has issued S tile n.
+__device__ __forceinline__ void wait_turn(volatile uint32_t* turns, int x, uint32_t n, volatile int* dead) {
+  for (int i = 0; turns[x ^ 1] < n + x && !*dead && i < kMaxPolls; ++i) __nanosleep(20);
+}
+// Shared-memory descriptors from their low word's address (see umma_desc_k_sw128, umma_desc_mn_sw128).
+__device__ __forceinline__ uint64_t desc_k(uint32_t addr16) {
+  return ((uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32) | (addr16 | (1u << 16));
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t addr16, uint32_t lbo16) {
+  return ((uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32) | (addr16 | (lbo16 << 16));
+}
+__device__ __forceinline__ bool elect_one() {
+  uint32_t ok;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(ok));
+  return ok != 0;
+}
+
+// The CTA's pieces, listed ahead in shared memory by one thread (a role that walked the line itself would
+// carry its state in registers and wait for the tables at every piece). Every role reads every piece, and an
+// entry is written anew once all have copied it. These waits outlast the others and do not give up with them
+// when the CTA is dead: no role waits for anything else then, so all arrive here, and every warp sees the
+// same pieces (the barriers among a stream's four warps depend on nothing but the piece).
+__device__ __forceinline__ void mbar_wait_long(uint64_t* bar, uint32_t parity) {
+  for (int i = 0; i < 8; ++i)
+    if (mbar_wait(bar, parity)) return;
+}
+struct PieceRing {
+  const Piece* e;
+  uint64_t *full, *empty;
+  uint32_t k;
+  // Copies the next piece; false after the last. `lanes`: the threads of the warp that read it.
+  __device__ __forceinline__ bool next(Piece& p, uint32_t lanes, bool first) {
+    mbar_wait_long(&full[k % kPieces], (k / kPieces) & 1);
+    p = e[k % kPieces];
+    __syncwarp(lanes);
+    if (first) mbar_arrive(&empty[k % kPieces]);
+    ++k;
+    return p.kt1 > p.kt0;
+  }
+};
+
+// What a stream does with a piece.
+enum { kSkip = 0, kHalf, kEvery2nd, kTransposed };
+struct Part {
+  int mode, rows, row_at, nr;  // rows of the piece, this stream's first row and its rows
+  int first, step, tiles;      // its key tiles: first, first + step, ... < tiles
+};
+__device__ __forceinline__ Part piece_part(const Piece& p, int G, int x, uint32_t turn) {
+  Part t;
+  t.rows = p.ntok * G;
+  t.tiles = p.kt1 - p.kt0;
+  t.row_at = 0;
+  t.nr = t.rows;
+  t.first = 0;
+  t.step = 1;
+  if (t.rows > 128) {
+    t.mode = kHalf;
+    t.row_at = x * 128;
+    t.nr = min(t.rows - t.row_at, 128);
+  } else if (prefix_two_streams(t.rows)) {
+    t.mode = x < t.tiles ? kEvery2nd : kSkip;
+    t.first = x;
+    t.step = 2;
+  } else {
+    t.mode = (turn & 1) == (uint32_t)x ? kTransposed : kSkip;
+  }
+  return t;
+}
+// Rows of the transposed MMAs' N for nr rows, and the values a softmax thread holds.
+__device__ __forceinline__ int t_cols(int nr) { return nr <= 16 ? 16 : nr <= 32 ? 32 : 64; }
+
+// State of one softmax stream while it works on a piece.
+struct Soft {
+  const PrefixArgs& a;
+  const LineShape& ls;
+  const Piece& p;
+  const Part& t;
+  unsigned char* smem;
+  uint64_t *full, *s_full, *p_ready, *pv_done, *both;
+  volatile uint32_t* armed;
+  volatile int* dead;
+  int* poison;  // this piece's flag
+  float sc;
+  uint32_t base;  // ring position of the piece
+  int x, r, lane, warp4;
+  uint32_t tS, tO;
+  uint32_t& meets;  // meetings of the two streams so far
+  // The two streams of a tall row tile meet.
+  __device__ __forceinline__ void meet() const {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(both);
+    wait_bar(both, meets & 1, dead, a.status);
+    ++meets;
+  }
+};
+
+// The prefix mask of a key tile: bits of this warp's 32 V rows and, for the row-wise softmax, of all 128.
+__device__ __forceinline__ bool tile_mask(const Soft& f, int k0, uint32_t* w, uint32_t& wr) {
+  wr = ~0u;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) w[j] = ~0u;
+  if (!f.a.mask || f.p.own) return false;
+  bool masked = false;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int key = k0 + j * 32 + f.lane;
+    w[j] = __ballot_sync(0xffffffffu, key < f.p.kend && f.a.mask[key] != 0);
+    masked |= w[j] != ~0u;
+    if (j == f.warp4) wr = w[j];
+  }
+  return masked;
+}
+
+// V rows that no row here attends (masked, behind the end, absent) may hold anything: they become zeros,
+// since the MMA multiplies them by 0. Values hidden from the first rows and attended by the last that are
+// not finite are taken out here and added to the rows that attend them at the end of the piece. Returns
+// whether the piece has any of those.
+template <int DT, int D>
+__device__ __forceinline__ bool clean_v(const Soft& f, int i, int k0, bool masked, uint32_t wr, bool any) {
+  using T = typename Elem<DT>::T;
+  using SM = MmaSmem<D>;
+  const bool scan = f.p.own && f.p.c0 + 1 < f.p.kend && k0 + kMmaK > f.p.c0 + 1;
+  if (!(masked || (f.p.own && k0 + kMmaK > f.p.kend) || scan)) return any;
+  const uint32_t nv = f.base + 2 * i + 1;
+  wait_full<SM::NB>(f.full, nv, f.armed, f.dead, f.a.status);
+  unsigned char* sV = f.smem + SM::ring + (nv % SM::NB) * SM::tile + f.r * 128;
+  const int key = k0 + f.r, rot = f.r & 7;  // chunks in an order that spreads a warp over the banks
+  const bool half = f.t.mode == kHalf;
+  if (key >= f.p.kend || !(wr >> f.lane & 1u)) {
+#pragma unroll
+    for (int c = 0; c < SM::PL * 8; ++c)
+      *reinterpret_cast<uint4*>(sV + (c >> 3) * 16384 + (((c & 7) ^ rot) << 4)) = make_uint4(0u, 0u, 0u, 0u);
+  } else if (scan && key > f.p.c0 && (!half || f.x == 0)) {
+    bool odd = false;
+#pragma unroll 2
+    for (int c = 0; c < SM::PL * 8; ++c) {
+      uint4* at = reinterpret_cast<uint4*>(sV + (c >> 3) * 16384 + (((c & 7) ^ rot) << 4));
+      const uint4 u = *at;
+      float v[8];
+      unpack16<DT>(u, v);
+      bool bad = false;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) bad |= !isfinite(v[e]);
+      if (bad) {
+        odd = true;
+        alignas(16) T z[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) z[e] = Elem<DT>::from_f(isfinite(v[e]) ? v[e] : 0.f);
+        *at = *reinterpret_cast<uint4*>(z);
+      }
+    }
+    if (odd) atomicOr(f.poison, 1);
+  }
+  fence_proxy_async_smem();
+  if (scan) {
+    if (half) f.meet();
+    else named_sync(1 + f.x, 128);
+    any |= *reinterpret_cast<volatile int*>(f.poison) != 0;
+  }
+  return any;
+}
+
+// Calls fn(key, row of V) for the own keys of this stream's tiles in [c0 + 1, lim).
+template <int DT, int D, typename F>
+__device__ __forceinline__ void hidden_rows(const Soft& f, int lim, F fn) {
+  using T = typename Elem<DT>::T;
+  const int sh = __ffs(f.a.page_size) - 1;
+  for (int i = f.t.first; i < f.t.tiles; i += f.t.step) {
+    const int k0 = (f.p.kt0 + i) * kMmaK;
+    for (int key = max(k0, f.p.c0 + 1); key < min(k0 + kMmaK, lim); ++key) {
+      const int page = f.a.block_table[(size_t)f.p.b * f.a.max_blocks + (key >> sh)];
+      if (page >= 0 && page < f.a.n_pages)
+        fn(key, reinterpret_cast<const T*>(f.a.v_pages) +
+                    (((size_t)page * f.ls.Hk + f.p.h) * f.a.page_size + (key & (f.a.page_size - 1))) * D);
+    }
+  }
+}
+
+// A thread per row: the key tiles of the piece. nt counts the stream's tiles.
+template <int DT, int D>
+__device__ __forceinline__ void rows_tiles(const Soft& f, uint32_t& nt, float& m, float& l, bool& any) {
+  const Piece& p = f.p;
+  const bool live = f.warp4 * 32 < f.t.nr;  // of a warp without rows nothing is read
+  const int lg = __ffs(f.ls.G) - 1;
+  const int lim = p.own ? min(p.c0 + ((f.t.row_at + f.r) >> lg) + 1, p.kend) : p.kend;  // keys this row sees
+  for (int i = f.t.first; i < f.t.tiles; i += f.t.step, ++nt) {
+    const int k0 = (p.kt0 + i) * kMmaK;
+    uint32_t w[4], wr;
+    const bool masked = tile_mask(f, k0, w, wr);
+    wait_bar(f.s_full, nt & 1, f.dead, f.a.status);
+    tc_fence_after();
+    if (live) {
+      const int n = lim - k0;  // columns seen
+      const bool edge = masked || __any_sync(0xffffffffu, n < kMmaK);
+      // 32 columns at a time, in loops that stay loops: S is read from TMEM twice, and the code of a tile is
+      // a few kilobytes (unrolled over 128 columns it ran from instruction cache misses: measured 3.9 us for
+      // a tile of 256 rows)
+      auto load = [&](int j, float* s) {
+        tmem_ld_x32(f.tS + j * 32, s);
+        tmem_wait_ld();
+        if (edge) {
+          const int c = n - j * 32;
+          uint32_t seen = j == 0 ? w[0] : j == 1 ? w[1] : j == 2 ? w[2] : w[3];
+          seen &= c >= 32 ? ~0u : c <= 0 ? 0u : (1u << c) - 1u;
+#pragma unroll
+          for (int e = 0; e < 32; ++e) s[e] = seen >> e & 1u ? s[e] : kNegInf;
+        }
+      };
+      float mx0 = kNegInf, mx1 = kNegInf;
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j) {
+        float s[32];
+        load(j, s);
+#pragma unroll
+        for (int e = 0; e < 32; e += 4) {
+          mx0 = fmaxf(mx0, fmaxf(s[e], s[e + 1]));
+          mx1 = fmaxf(mx1, fmaxf(s[e + 2], s[e + 3]));
+        }
+      }
+      const float mt = fmaxf(mx0, mx1) * f.sc;
+      if (__any_sync(0xffffffffu, f.r < f.t.nr && mt > m + kLazy)) {  // rows of no token hold anything: no vote
+        const float mn = fmaxf(m, mt), al = ex2_approx(m - (mn == kNegInf ? 0.f : mn));
+        m = mn;
+        l *= al;
+        if (i > f.t.first) {
+#pragma unroll 1
+          for (int j = 0; j < D; j += 32) {
+            float o[32];
+            tmem_ld_x32(f.tO + j, o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] *= al;
+            tmem_st_x32(f.tO + j, o);
+          }
+        }
+      }
+      const float ref = m == kNegInf ? 0.f : m;
+      float l0 = 0.f, l1 = 0.f;
+#pragma unroll 1
+      for (int j = 0; j < 4; ++j) {
+        float s[32];
+        load(j, s);
+        uint32_t pk[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float p0 = ex2_approx(fmaf(s[2 * e], f.sc, -ref));
+          const float p1 = ex2_approx(fmaf(s[2 * e + 1], f.sc, -ref));
+          l0 += p0;
+          l1 += p1;
+          pk[e] = pack2<DT>(p0, p1);
+        }
+        tmem_st_x16(f.tS + j * 16, pk);
+      }
+      l += l0 + l1;
+      tmem_wait_st();
+    }
+    any = clean_v<DT, D>(f, i, k0, masked, wr, any);
+    tc_fence_before();
+    __syncwarp();
+    if (f.lane == 0) mbar_arrive(f.p_ready);
+  }
+}
+
+template <int DT, int D>
+__device__ __forceinline__ void rows_out(const Soft& f, float m, float l, bool any, float2* ml, float* part) {
+  const Piece& p = f.p;
+  const int nr = f.t.nr, lg = __ffs(f.ls.G) - 1;
+  const int64_t blk = p.row0 + (f.t.mode == kHalf ? f.x * 128 : f.x * f.t.rows);
+  if (f.warp4 * 32 < nr) {
+    const int lim = p.own ? min(p.c0 + ((f.t.row_at + f.r) >> lg) + 1, p.kend) : p.kend;
+#pragma unroll 1
+    for (int j = 0; j < D; j += 32) {
+      float o[32];
+      tmem_ld_x32(f.tO + j, o);
+      tmem_wait_ld();
+      if (any && f.r < nr)
+        hidden_rows<DT, D>(f, lim, [&](int, const typename Elem<DT>::T* v) {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) {
+            const float y = Elem<DT>::to_f(v[j + e]);
+            if (!isfinite(y)) o[e] += y;
+          }
+        });
+      if (f.r < nr) {
+        float4* dst = reinterpret_cast<float4*>(part + (size_t)blk * D) + (size_t)(j / 4) * nr + f.r;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) dst[(size_t)e * nr] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+      }
+    }
+  }
+  if (f.r < nr) ml[blk + f.r] = make_float2(m, l);
+}
+
+// A thread per key: the key tiles of a piece of up to N rows, and its maxima and sums.
+template <int DT, int D, int N>
+__device__ __forceinline__ bool cols_tiles(const Soft& f, uint32_t& nt, float2* ml) {
+  using T = typename Elem<DT>::T;
+  using SM = MmaSmem<D>;
+  constexpr int NQ = N < 16 ? 16 : N;  // rows of the operands
+  const Piece& p = f.p;
+  const int nr = f.t.nr, lane = f.lane;
+  float* red = reinterpret_cast<float*>(f.smem + SM::red) + f.x * 256;  // [4 warps][64]
+  unsigned char* sP = f.smem + f.x * SM::qbuf + SM::pt + (f.r >> 6) * (NQ * 128) + (f.r & 7) * 2;
+  const int chunk = (f.r & 63) >> 3;
+  // reference maxima: of row `lane`, and of row 32 + lane
+  float m0 = kNegInf, m1 = kNegInf, l[N];
+#pragma unroll
+  for (int n = 0; n < N; ++n) l[n] = 0.f;
+  bool any = false;
+  for (int i = 0; i < f.t.tiles; ++i, ++nt) {
+    const int k0 = (p.kt0 + i) * kMmaK, key = k0 + f.r;
+    uint32_t w[4], wr;
+    const bool masked = tile_mask(f, k0, w, wr);
+    const bool ok = key < p.kend && (wr >> lane & 1u);
+    // own key `key` is seen by the rows from (key - c0) G on
+    const int from = !ok ? N : p.own ? max(key - p.c0, 0) * f.ls.G : 0;
+    wait_bar(f.s_full, nt & 1, f.dead, f.a.status);
+    tc_fence_after();
+    float s[N];
+    tmem_ld_n<N>(f.tS, s);
+    float w0 = kNegInf, w1 = kNegInf;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      s[n] = n >= from ? s[n] : kNegInf;
+      const float y = redux_max(s[n]);
+      if (lane == (n & 31)) (n < 32 ? w0 : w1) = y;
+    }
+    if (lane < N) red[f.warp4 * 64 + lane] = w0;
+    if (N > 32) red[f.warp4 * 64 + 32 + lane] = w1;
+    named_sync(1 + f.x, 128);
+    // every warp finds the same maxima; the buffer is free again once all have arrived at p_ready
+    float t0 = kNegInf, t1 = kNegInf;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (lane < N) t0 = fmaxf(t0, red[j * 64 + lane]);
+      if (N > 32) t1 = fmaxf(t1, red[j * 64 + 32 + lane]);
+    }
+    t0 *= f.sc;
+    t1 *= f.sc;
+    const bool up = (lane < nr && t0 > m0 + kLazy) || (N > 32 && 32 + lane < nr && t1 > m1 + kLazy);
+    if (__any_sync(0xffffffffu, up)) {
+      const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
+      const float a0 = ex2_approx(m0 - (n0 == kNegInf ? 0.f : n0)), a1 = ex2_approx(m1 - (n1 == kNegInf ? 0.f : n1));
+      m0 = n0;
+      m1 = n1;
+#pragma unroll
+      for (int n = 0; n < N; ++n) l[n] *= __shfl_sync(0xffffffffu, n < 32 ? a0 : a1, n & 31);
+      if (i > 0) {
+#pragma unroll
+        for (int j = 0; j < N; j += 8) {
+          float o[8];
+          tmem_ld_x8(f.tO + j, o);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) o[e] *= __shfl_sync(0xffffffffu, j < 32 ? a0 : a1, (j + e) & 31);
+          tmem_st_x8(f.tO + j, o);
+        }
+        tmem_wait_st();
+      }
+    }
+    const float r0 = m0 == kNegInf ? 0.f : m0, r1 = m1 == kNegInf ? 0.f : m1;
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+      const float pr = ex2_approx(fmaf(s[n], f.sc, -__shfl_sync(0xffffffffu, n < 32 ? r0 : r1, n & 31)));
+      l[n] += pr;
+      *reinterpret_cast<T*>(sP + n * 128 + ((chunk ^ (n & 7)) << 4)) = Elem<DT>::from_f(pr);
+    }
+    fence_proxy_async_smem();
+    any = clean_v<DT, D>(f, i, k0, masked, wr, any);
+    tc_fence_before();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(f.p_ready);
+  }
+  // sums over the keys: a warp's, then the four warps' (every warp has read the last tile's maxima)
+  float w0 = 0.f, w1 = 0.f;
+#pragma unroll
+  for (int n = 0; n < N; ++n) {
+    const float y = warp_sum(l[n]);
+    if (lane == (n & 31)) (n < 32 ? w0 : w1) = y;
+  }
+  named_sync(1 + f.x, 128);
+  if (lane < N) red[f.warp4 * 64 + lane] = w0;
+  if (N > 32) red[f.warp4 * 64 + 32 + lane] = w1;
+  named_sync(1 + f.x, 128);
+  if (f.r < nr)
+    ml[p.row0 + f.r] = make_float2(f.r < 32 ? m0 : m1, red[f.r] + red[64 + f.r] + red[128 + f.r] + red[192 + f.r]);
+  return any;
+}
+
+template <int DT, int D, int N>
+__device__ __forceinline__ void cols_out(const Soft& f, bool any, float* part) {
+  using T = typename Elem<DT>::T;
+  const Piece& p = f.p;
+  const int nr = f.t.nr;
+  if (f.r < D) {  // thread = output column; whole warps
+    float o[N];
+    tmem_ld_n<N>(f.tO, o);
+    if (any)
+      hidden_rows<DT, D>(f, p.kend, [&](int key, const T* v) {
+        const float y = Elem<DT>::to_f(v[f.r]);
+        if (!isfinite(y))
+#pragma unroll
+          for (int n = 0; n < N; ++n)
+            if (n >= (key - p.c0) * f.ls.G) o[n] += y;
+      });
+    float* dst = part + (size_t)p.row0 * D + (size_t)(f.r >> 2) * nr * 4 + (f.r & 3);
+#pragma unroll
+    for (int n = 0; n < N; ++n)
+      if (n < nr) dst[n * 4] = o[n];
+  }
+}
+
 template <int DT, int D>
 __global__ void __launch_bounds__(kMmaThreads, 1)
     prefix_mma_kernel(PrefixArgs a, LineShape ls, int64_t* hdr, float2* ml, float* part, const __grid_constant__ PrefixMaps maps) {
@@ -142,21 +589,28 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   using SM = MmaSmem<D>;
   constexpr int PL = SM::PL, NB = SM::NB;
   constexpr uint32_t kFmt = DT == HC_BF16 ? 1u : 0u;
-  constexpr uint32_t kIdS = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((uint32_t)(kMmaK >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-  // P V: N = D, B (V) MN-major
-  constexpr uint32_t kIdO = (1u << 4) | (kFmt << 7) | (kFmt << 10) | (1u << 16) | ((uint32_t)(D >> 3) << 17) |
-                            ((uint32_t)(128 >> 4) << 24);
+  constexpr uint32_t kId = (1u << 4) | (kFmt << 7) | (kFmt << 10) | ((uint32_t)(128 >> 4) << 24);  // fp32 sums, M = 128
+  constexpr uint32_t kIdS = kId | ((uint32_t)(kMmaK >> 3) << 17);
+  constexpr uint32_t kIdO = kId | (1u << 16) | ((uint32_t)(D >> 3) << 17);  // N = D, B (V) MN-major
   extern __shared__ __align__(1024) unsigned char smem[];
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + SM::bars);
   uint64_t *empty = full + NB, *s_full = empty + NB, *p_ready = s_full + 2, *pv_done = p_ready + 2, *q_ready = pv_done + 2;
   uint64_t* fin = q_ready + 2;
   uint32_t* s_tmem = reinterpret_cast<uint32_t*>(smem + SM::misc);
   volatile int* dead = reinterpret_cast<volatile int*>(smem + SM::misc + 4);
-  int* poison = reinterpret_cast<int*>(smem + SM::misc + 8);  // per stream: a hidden value was not finite
-  volatile uint32_t* armed = reinterpret_cast<volatile uint32_t*>(smem + SM::misc + 16);  // ring positions armed
+  volatile uint32_t* armed = reinterpret_cast<volatile uint32_t*>(smem + SM::misc + 8);  // ring positions armed
+  uint64_t* both = fin + 1;
+  volatile uint32_t* turns = armed + 5;  // per stream: S tiles of tall row tiles issued
+  int* poison = reinterpret_cast<int*>(smem + SM::misc + 16);  // a hidden value was not finite: per stream, and both halves'
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = ls.G;
+  PieceRing ring{reinterpret_cast<const Piece*>(smem + SM::pieces), reinterpret_cast<uint64_t*>(smem + SM::pbars),
+                 reinterpret_cast<uint64_t*>(smem + SM::pbars) + kPieces, 0};
 
   if (tid == 0) {
+    for (int i = 0; i < kPieces; ++i) {
+      mbar_init(&ring.full[i], 1);
+      mbar_init(&ring.empty[i], 11);  // producer, two issuers, eight softmax warps
+    }
     for (int i = 0; i < NB; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 2);
@@ -168,10 +622,12 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       mbar_init(&q_ready[x], 4);
     }
     mbar_init(fin, 2);
+    mbar_init(both, 8);
     fence_mbar_init();
     *dead = 0;
     *armed = 0;
-    poison[0] = poison[1] = 0;
+    poison[0] = poison[1] = poison[2] = 0;
+    turns[0] = turns[1] = 0;
     prefetch_tensormap(&maps.kp);
     prefetch_tensormap(&maps.vp);
     if (ls.P > 0) {
@@ -186,10 +642,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   const uint32_t tbase = *s_tmem;
   pdl_wait();
   const LineGeom g(ls, min(a.T, max(a.cu_new[ls.n_seq], 0)));
-  LineWalk walk;
-  walk.c = blockIdx.x;
-  walk.st = line_setup<kMmaThreads>(a, ls, g, blockIdx.x, hdr, reinterpret_cast<int64_t*>(smem + SM::scan));
-  Piece p;
+  const Stretch st = line_setup<kMmaThreads>(a, ls, g, blockIdx.x, hdr, reinterpret_cast<int64_t*>(smem + SM::red));
+  __syncthreads();  // the setup's buffer is used anew
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
@@ -199,11 +653,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       const int bx = min(a.page_size, kMmaK), nbx = kMmaK / bx;
       const int y_out = a.n_pages * ls.Hk * a.page_size;  // out of range: reads as zeros
       uint32_t n = 0;
-      bool stop = false;
-      while (!stop && walk.next(a, ls, g, p)) {
+      Piece p;
+      while (ring.next(p, 0xffffffffu, lane == 0)) {
         for (int kt = p.kt0; kt < p.kt1; ++kt) {
-          stop = __any_sync(0xffffffffu, *dead);
-          if (stop) break;
+          if (__any_sync(0xffffffffu, *dead)) break;
           int y = y_out;
           if (p.own && lane < nbx) {
             const int key = kt * kMmaK + lane * bx;
@@ -239,239 +692,184 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       // copies still in flight write this CTA's shared memory: they land before it ends
       for (uint32_t i = n > NB ? n - NB : 0; i < n; ++i) mbar_wait(&full[i % NB], (i / NB) & 1);
     } else if (warp < 3) {
-      // ---- MMA issue of stream x ---------------------------------------------------------
-      if (lane == 0) {
-        const int x = warp - 1;
-        const uint32_t tS = tbase + x * 128, tO = tbase + 256 + x * 128;
-        const uint32_t sq = smem_u32(smem + SM::q + x * SM::tile), sr = smem_u32(smem + SM::ring);
-        uint32_t base = 0, np = 0, nt = 0;  // ring position, pieces and tiles of this stream
-        while (walk.next(a, ls, g, p)) {
-          const bool both = p.ntok * G > 128;
-          const int tiles = p.kt1 - p.kt0, step = both ? 1 : 2;
-          bool begun = false;
-          for (int i = both ? 0 : x; i < tiles; i += step, ++nt) {
+      // ---- MMA issue of stream x: the warp walks together, one thread issues ----------------
+      const int x = warp - 1;
+      const bool leader = elect_one();
+      const uint32_t tS = tbase + x * 128, tO = tbase + 256 + x * 128;
+      // low words of the operands' descriptors (address / 16), stepped by adding
+      const uint32_t dq = smem_u32(smem + x * SM::qbuf) >> 4, dr = smem_u32(smem + SM::ring) >> 4;
+      uint32_t base = 0, np = 0, nt = 0, turn = 0, tall = 0;  // ring position; pieces, tiles, tall tiles of this stream
+      Piece p;
+      while (ring.next(p, 0xffffffffu, lane == 0)) {
+        const Part t = piece_part(p, G, x, turn);
+        if (t.rows <= 64) ++turn;
+        if (t.mode != kSkip) {
+          const bool tr = t.mode == kTransposed, half = t.mode == kHalf;
+          const uint32_t nq = t_cols(t.nr), idt = kId | ((nq >> 3) << 17);
+          wait_bar(&q_ready[x], np & 1, dead, a.status);
+          ++np;
+          for (int i = t.first; i < t.tiles; i += t.step, ++nt) {
             const uint32_t nk = base + 2 * i, nv = nk + 1, bk = nk % NB, bv = nv % NB;
-            if (!begun) wait_bar(&q_ready[x], np & 1, dead, a.status);
+            const uint32_t dk = dr + bk * (SM::tile >> 4), dv = dr + bv * (SM::tile >> 4);
             wait_full<NB>(full, nk, armed, dead, a.status);
             if (nt > 0) wait_bar(&pv_done[x], (nt - 1) & 1, dead, a.status);  // P of the last tile has been read
+            if (half && i == 0) wait_turn(turns, x, tall, dead);
             tc_fence_after();
+            if (leader) {
+              if (tr) {
 #pragma unroll
-            for (int ks = 0; ks < D / 16; ++ks)
-              umma_f16(tS, umma_desc_k_sw128(sq + (ks >> 2) * 16384u + (ks & 3) * 32u),
-                       umma_desc_k_sw128(sr + bk * SM::tile + (ks >> 2) * 16384u + (ks & 3) * 32u), kIdS, ks > 0);
-            umma_commit(&s_full[x]);
-            umma_commit(&empty[bk]);
-            if (!both) umma_commit(&empty[bk]);
-            wait_bar(&p_ready[x], nt & 1, dead, a.status);
+                for (int ks = 0; ks < D / 16; ++ks)
+                  umma_f16(tS, desc_k(dk + (ks >> 2) * 1024 + (ks & 3) * 2), desc_k(dq + (ks >> 2) * nq * 8 + (ks & 3) * 2), idt,
+                           ks > 0);
+              } else {
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
+                  umma_f16(tS, desc_k(dq + (ks >> 2) * 1024 + (ks & 3) * 2), desc_k(dk + (ks >> 2) * 1024 + (ks & 3) * 2), kIdS,
+                           ks > 0);
+              }
+              umma_commit(&s_full[x]);
+              if (half) turns[x] = tall + 1;
+              umma_commit(&empty[bk]);
+              if (!half) umma_commit(&empty[bk]);  // the tile is this stream's alone
+            }
+            if (half) ++tall;
             wait_full<NB>(full, nv, armed, dead, a.status);
+            wait_bar(&p_ready[x], nt & 1, dead, a.status);
+            // The two halves of a tall row tile take turns, [O += P V, next S] each: mixed with one another
+            // they would finish together, and then both softmaxes run while the tensor cores wait.
+            if (half && i + 1 < t.tiles) wait_turn(turns, x, tall, dead);
             tc_fence_after();
+            if (leader) {
+              const uint32_t more = i > t.first;
+              if (tr) {
+                // A = V^T from its MN-major rows. M is 128: for D = 64 the same plane serves as both halves
+                // (a plane stride of 0) and the lower half of the result is not read
+                const uint32_t dp = dq + (SM::pt >> 4);
 #pragma unroll
-            for (int ks = 0; ks < kMmaK / 16; ++ks)
-              umma_f16_ts(tO, tS + ks * 8, umma_desc_mn_sw128(sr + bv * SM::tile + ks * 2048u, 16384u), kIdO,
-                          (begun || ks > 0) ? 1u : 0u);
-            umma_commit(&pv_done[x]);
-            umma_commit(&empty[bv]);
-            if (!both) umma_commit(&empty[bv]);
-            begun = true;
+                for (int ks = 0; ks < kMmaK / 16; ++ks)
+                  umma_f16(tO, desc_mn(dv + ks * 128, D == 128 ? 1024 : 0), desc_k(dp + (ks >> 2) * nq * 8 + (ks & 3) * 2),
+                           idt | (1u << 15), more | (ks > 0));
+              } else {
+#pragma unroll
+                for (int ks = 0; ks < kMmaK / 16; ++ks)
+                  umma_f16_ts(tO, tS + ks * 8, desc_mn(dv + ks * 128, 1024), kIdO, more | (ks > 0));
+              }
+              umma_commit(&pv_done[x]);
+              umma_commit(&empty[bv]);
+              if (!half) umma_commit(&empty[bv]);
+            }
+            __syncwarp();
           }
-          if (begun) ++np;
-          base += 2 * tiles;
         }
-        umma_commit(fin);
+        base += 2 * t.tiles;
       }
-      __syncwarp();
+      if (leader) umma_commit(fin);
+    } else if (lane == 0) {
+      // ---- lists the pieces --------------------------------------------------------------
+      LineWalk walk(a, ls, g, st, blockIdx.x);
+      Piece* out = reinterpret_cast<Piece*>(smem + SM::pieces);
+      Piece p{};
+      bool more = true;
+      for (uint32_t k = 0; more; ++k) {
+        more = walk.next(a, ls, g, p);
+        if (!more) p.kt0 = p.kt1 = 0;  // the end
+        mbar_wait_long(&ring.empty[k % kPieces], ((k / kPieces) & 1) ^ 1);
+        out[k % kPieces] = p;
+        mbar_arrive(&ring.full[k % kPieces]);
+      }
     }
+    __syncwarp();
   } else {
-    // ---- softmax of stream x: thread = row -------------------------------------------------
+    // ---- softmax of stream x ---------------------------------------------------------------
     asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
-    const int x = (warp >> 2) - 1, r = tid & 127;
-    const uint32_t quarter = (uint32_t)((warp & 3) * 32) << 16;
-    const uint32_t tS = tbase + x * 128 + quarter, tO = tbase + 256 + x * 128 + quarter;
-    unsigned char* sQ = smem + SM::q + x * SM::tile;
-    const float sc = a.scale * 1.4426950408889634f;
-    uint32_t base = 0, nt = 0;
-    while (walk.next(a, ls, g, p)) {
-      const int rows = p.ntok * G, tiles = p.kt1 - p.kt0;
-      const bool both = rows > 128;
-      const int row_at = both ? x * 128 : 0;                 // this stream's first row of the row tile
-      const int nr = min(max(rows - row_at, 0), 128);
-      const int64_t out_row = p.row0 + (both ? x * 128 : x * rows) + r;
-      const int first = both ? 0 : x, step = both ? 1 : 2;
+    const int x = (warp >> 2) - 1, r = tid & 127, warp4 = warp & 3, lg = __ffs(G) - 1;
+    const uint32_t quarter = (uint32_t)(warp4 * 32) << 16;
+    unsigned char* sQ = smem + x * SM::qbuf;
+    uint32_t base = 0, next_base = 0, nt = 0, turn = 0, meets = 0;
+    Piece p, q;
+    Part tq;
+    // the next piece of this stream; `base` goes along
+    auto advance = [&]() -> bool {
+      for (;;) {
+        if (!ring.next(q, 0xffffffffu, lane == 0)) return false;
+        tq = piece_part(q, G, x, turn);
+        base = next_base;
+        next_base += 2 * tq.tiles;
+        if (tq.rows <= 64) ++turn;
+        if (tq.mode != kSkip) return true;
+        // too few key tiles for this stream: its block of partial rows holds nothing
+        if (prefix_two_streams(tq.rows) && r < tq.rows) ml[q.row0 + tq.rows + r] = make_float2(kNegInf, 0.f);
+      }
+    };
+    // its Q rows: 16 bytes a thread at a time, all loads in flight, then into the swizzled K-major layout
+    constexpr int CPR = D / 8, QB = 128 * CPR / 128;
+    uint4 u[QB];
+    auto load_q = [&]() {
+      const int total = tq.nr * CPR;
+#pragma unroll
+      for (int j = 0; j < QB; ++j) {
+        const int k = r + j * 128, row = tq.row_at + k / CPR;
+        if (k < total)
+          u[j] = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (int64_t)(q.tok0 + (row >> lg)) * a.q_st +
+                                                (int64_t)(q.h * G + (row & (G - 1))) * a.q_sh)[k % CPR];
+      }
+    };
+    auto store_q = [&]() {
+      const int total = tq.nr * CPR;
+      const uint32_t plane = tq.mode == kTransposed ? t_cols(tq.nr) * 128u : 16384u;
+#pragma unroll
+      for (int j = 0; j < QB; ++j) {
+        const int k = r + j * 128, rr = k / CPR, c = k % CPR;
+        if (k < total) *reinterpret_cast<uint4*>(sQ + (c >> 3) * plane + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = u[j];
+      }
+      fence_proxy_async_smem();
+    };
+    auto q_arrive = [&]() {
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&q_ready[x]);
+    };
+    bool have = advance();
+    if (have) {
+      load_q();
+      store_q();
+      q_arrive();
+    }
+    while (have) {
+      p = q;
+      const Part t = tq;
+      const Soft f{a, ls, p, t, smem, full, &s_full[x], &p_ready[x], &pv_done[x], both, armed, dead,
+                   &poison[t.mode == kHalf ? 2 : x], a.scale * 1.4426950408889634f, base, x, r, lane, warp4,
+                   tbase + x * 128 + quarter, tbase + 256 + x * 128 + quarter, meets};
+      // The next piece's Q is loaded and its first MMAs begin while this one's result is written: all MMAs
+      // that read Q, P or S have ended, and O is only overwritten after the next p_ready.
       float m = kNegInf, l = 0.f;
-      if (first < tiles) {
-        // Q rows, 16 bytes a thread at a time, in the swizzled K-major layout
-        constexpr int CPR = D / 8;
-#pragma unroll 4
-        for (int k = r; k < 128 * CPR; k += 128) {
-          const int rr = k / CPR, c = k % CPR;
-          if (rr < nr) {
-            const int row = row_at + rr;
-            const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(p.tok0 + row / G) * a.q_st +
-                           (int64_t)(p.h * G + row % G) * a.q_sh;
-            *reinterpret_cast<uint4*>(sQ + (c >> 3) * 16384 + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) =
-                reinterpret_cast<const uint4*>(src)[c];
-          }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&q_ready[x]);
+      bool any = false;
+      const bool tr = t.mode == kTransposed;
+      if (!tr) rows_tiles<DT, D>(f, nt, m, l, any);
+      else if (t.nr <= 8) any = cols_tiles<DT, D, 8>(f, nt, ml);
+      else if (t.nr <= 16) any = cols_tiles<DT, D, 16>(f, nt, ml);
+      else if (t.nr <= 32) any = cols_tiles<DT, D, 32>(f, nt, ml);
+      else any = cols_tiles<DT, D, 64>(f, nt, ml);
+      have = advance();
+      if (have) load_q();
+      wait_bar(&pv_done[x], (nt - 1) & 1, dead, a.status);
+      tc_fence_after();
+      if (have) {
+        store_q();
+        q_arrive();
       }
-      const bool live = (warp & 3) * 32 < nr;  // of a warp without rows nothing is read
-      // own keys of this row: j < lim
-      const int lim = p.own ? min(p.c0 + (row_at + r) / G + 1, p.kend) : p.kend;
-      const bool hides = p.own && p.c0 + 1 < p.kend;  // some key here is hidden from some row
-      bool any_poison = false;
-      for (int i = first; i < tiles; i += step, ++nt) {
-        const int k0 = (p.kt0 + i) * kMmaK;
-        uint32_t w[4] = {~0u, ~0u, ~0u, ~0u};
-        uint32_t wr = ~0u;  // the word of this thread's V row
-        bool masked = false;
-        if (a.mask && !p.own) {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const int key = k0 + j * 32 + lane;
-            w[j] = __ballot_sync(0xffffffffu, key < p.kend && a.mask[key] != 0);
-            masked |= w[j] != ~0u;
-            if (j == (warp & 3)) wr = w[j];
-          }
-        }
-        wait_bar(&s_full[x], nt & 1, dead, a.status);
-        tc_fence_after();
-        if (live) {
-          float s[128];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) tmem_ld_x32(tS + j * 32, s + j * 32);
-          tmem_wait_ld();
-          const int n = lim - k0;  // columns seen
-          if (masked || __any_sync(0xffffffffu, n < kMmaK)) {
-#pragma unroll
-            for (int j = 0; j < 128; ++j) s[j] = j < n && (w[j >> 5] >> (j & 31) & 1u) ? s[j] : kNegInf;
-          }
-          float mx0 = s[0], mx1 = s[1], mx2 = s[2], mx3 = s[3];
-#pragma unroll
-          for (int j = 4; j < 128; j += 4) {
-            mx0 = fmaxf(mx0, s[j]);
-            mx1 = fmaxf(mx1, s[j + 1]);
-            mx2 = fmaxf(mx2, s[j + 2]);
-            mx3 = fmaxf(mx3, s[j + 3]);
-          }
-          const float mt = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3)) * sc;
-          if (__any_sync(0xffffffffu, r < nr && mt > m + kLazy)) {  // rows of no token hold anything: no vote
-            const float mn = fmaxf(m, mt), al = ex2_approx(m - (mn == kNegInf ? 0.f : mn));
-            m = mn;
-            l *= al;
-            if (i > first) {
-#pragma unroll
-              for (int j = 0; j < D; j += 32) {
-                float o[32];
-                tmem_ld_x32(tO + j, o);
-                tmem_wait_ld();
-#pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] *= al;
-                tmem_st_x32(tO + j, o);
-              }
-            }
-          }
-          const float ref = m == kNegInf ? 0.f : m;
-          float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            uint32_t pk[16];
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float p0 = ex2_approx(fmaf(s[j * 32 + 2 * e], sc, -ref));
-              const float p1 = ex2_approx(fmaf(s[j * 32 + 2 * e + 1], sc, -ref));
-              l0 += p0;
-              l1 += p1;
-              pk[e] = pack2<DT>(p0, p1);
-            }
-            tmem_st_x16(tS + j * 16, pk);
-          }
-          l += l0 + l1;
-          tmem_wait_st();
-        }
-        // V rows that no row here attends (masked, behind the end, absent) may hold anything: they become
-        // zeros, since the MMA multiplies them by 0
-        const uint32_t nv = base + 2 * i + 1, bv = nv % NB;
-        const bool scan = hides && k0 + kMmaK > p.c0 + 1;
-        if (masked || (p.own && k0 + kMmaK > p.kend) || scan) {
-          wait_full<NB>(full, nv, armed, dead, a.status);
-          unsigned char* sV = smem + SM::ring + bv * SM::tile + r * 128;
-          const int key = k0 + r;
-          if (key >= p.kend || !(wr >> lane & 1u)) {
-#pragma unroll
-            for (int c = 0; c < PL * 8; ++c) *reinterpret_cast<uint4*>(sV + (c >> 3) * 16384 + (c & 7) * 16) = make_uint4(0u, 0u, 0u, 0u);
-          } else if (scan && key > p.c0 && (!both || x == 0)) {
-            // hidden from the first rows and attended by the last: values that are not finite are taken
-            // out here and added to the rows that attend them at the end
-            bool odd = false;
-            for (int c = 0; c < PL * 8; ++c) {
-              uint4* at = reinterpret_cast<uint4*>(sV + (c >> 3) * 16384 + (c & 7) * 16);
-              uint4 u = *at;
-              float f[8];
-              unpack16<DT>(u, f);
-              bool bad = false;
-              for (int e = 0; e < 8; ++e) bad |= !isfinite(f[e]);
-              if (bad) {
-                odd = true;
-                alignas(16) T t[8];
-                for (int e = 0; e < 8; ++e) t[e] = Elem<DT>::from_f(isfinite(f[e]) ? f[e] : 0.f);
-                *at = *reinterpret_cast<uint4*>(t);
-              }
-            }
-            if (odd) atomicOr(&poison[x], 1);
-          }
-          fence_proxy_async_smem();
-          if (scan) {
-            named_sync(both ? 3 : 1 + x, both ? 256 : 128);
-            any_poison |= *reinterpret_cast<volatile int*>(&poison[both ? 0 : x]) != 0;
-          }
-        }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_ready[x]);
-      }
-      if (first < tiles) {
-        wait_bar(&pv_done[x], (nt - 1) & 1, dead, a.status);
-        tc_fence_after();
-        if (live) {
-          const T* vp = reinterpret_cast<const T*>(a.v_pages);
-          const int sh = __ffs(a.page_size) - 1;
-#pragma unroll
-          for (int j = 0; j < D; j += 32) {
-            float o[32];
-            tmem_ld_x32(tO + j, o);
-            tmem_wait_ld();
-            if (any_poison && r < nr) {
-              for (int i = first; i < tiles; i += step) {
-                const int k0 = (p.kt0 + i) * kMmaK;
-                for (int key = max(k0, p.c0 + 1); key < min(k0 + kMmaK, lim); ++key) {
-                  const int page = a.block_table[(size_t)p.b * a.max_blocks + (key >> sh)];
-                  if (page < 0 || page >= a.n_pages) continue;
-                  const T* v = vp + (((size_t)page * ls.Hk + p.h) * a.page_size + (key & (a.page_size - 1))) * D + j;
-#pragma unroll
-                  for (int e = 0; e < 32; ++e) {
-                    const float f = Elem<DT>::to_f(v[e]);
-                    if (!isfinite(f)) o[e] += f;
-                  }
-                }
-              }
-            }
-            if (r < nr) {
-              float4* dst = reinterpret_cast<float4*>(part + (size_t)out_row * D + j);
-#pragma unroll
-              for (int e = 0; e < 8; ++e) dst[e] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-            }
-          }
-        }
-        tc_fence_before();
-      }
-      if (r < nr) ml[out_row] = make_float2(m, l);
-      base += 2 * tiles;
-      if (any_poison) {  // cleared for the next piece once every thread that reads it has
-        named_sync(both ? 3 : 1 + x, both ? 256 : 128);
-        if (r == 0) poison[both ? 0 : x] = 0;
-        named_sync(both ? 3 : 1 + x, both ? 256 : 128);
+      if (!tr) rows_out<DT, D>(f, m, l, any, ml, part);
+      else if (t.nr <= 8) cols_out<DT, D, 8>(f, any, part);
+      else if (t.nr <= 16) cols_out<DT, D, 16>(f, any, part);
+      else if (t.nr <= 32) cols_out<DT, D, 32>(f, any, part);
+      else cols_out<DT, D, 64>(f, any, part);
+      tc_fence_before();
+      if (p.own && p.c0 + 1 < p.kend) {  // the flag is cleared once every thread has read it
+        if (t.mode == kHalf) f.meet();
+        else named_sync(1 + x, 128);
+        if (r == 0) *f.poison = 0;
+        if (t.mode == kHalf) f.meet();
+        else named_sync(1 + x, 128);
       }
     }
   }

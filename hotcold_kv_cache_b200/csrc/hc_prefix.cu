@@ -265,9 +265,10 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(PrefixArgs 
     if (lane < s.nch && g.ktp > 0) {
       const int i = t / g.tt, tok0 = i * g.tt;
       const int tiles = min(g.ct, g.ktp - lane * g.ct);
-      const int64_t v0 = h * g.head + (int64_t)lane * g.nrt * (g.ct + kOver) + (int64_t)i * (tiles + kOver);
+      const int64_t v0 = h * g.head + (int64_t)lane * g.nrt * (g.ct * g.pre.a + g.pre.b) +
+                         (int64_t)i * (tiles * g.pre.a + g.pre.b) + g.pre.b;
       rows = min(g.tt, R - tok0) * s.G, q0 = (t - tok0) * s.G;
-      lo = line_div(v0 + kOver, W), hi = line_div(v0 + kOver + tiles - 1, W);
+      lo = line_div(v0, W), hi = line_div(v0 + (int64_t)(tiles - 1) * g.pre.a, W);
       row = s.dup * (((int64_t)h * s.nch + lane) * s.T + tok0) * s.G;
     } else if (lane == s.nch && s_b >= 0) {
       const SeqLens q = seq_lens(a, s_b);
@@ -275,8 +276,9 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(PrefixArgs 
       const int tiles = ceil_div(seq_keys(q, tok1), s.kt);
       rows = (tok1 - r * g.tt) * s.G, q0 = (t - q.cu - r * g.tt) * s.G;
       if (tiles > 0) {
-        const int64_t v0 = hdr[1 + s_b] + ((int64_t)h * nr + r) * g.seq_group(s, q);
-        lo = line_div(v0 + kOver, W), hi = line_div(v0 + kOver + tiles - 1, W);
+        const LineCost k = line_cost(s, min(q.n * s.G, s.rt));
+        const int64_t v0 = hdr[1 + s_b] + ((int64_t)h * nr + r) * g.seq_group(s, q) + k.b;
+        lo = line_div(v0, W), hi = line_div(v0 + (int64_t)(tiles - 1) * k.a, W);
         row = s.dup * ((int64_t)s.Hk * s.T * (s.P > 0 ? s.nch : 0) + (int64_t)q.cu * s.Hk + (int64_t)h * q.n + r * g.tt) * s.G;
       }
     }

@@ -5,9 +5,9 @@
 // group) of the whole batch are stacked into row tiles and each prefix key tile is read once per row
 // tile, not once per sequence. The own-pages part has row tiles per sequence. A group is
 //   prefix: (KV head, chunk of key tiles, row tile)      suffix: (sequence, KV head, row tile)
-// and all groups lie one behind the other on a line, each as long as its key tiles plus kOver (the
-// cost of starting one). CTA c works on the stretch [c W, (c + 1) W) of the line: whatever the lengths,
-// every CTA gets the same number of key tiles, and where a stretch ends inside a group the group's rows
+// and all groups lie one behind the other on a line, each as long as it takes (line_cost: so much to start
+// it and so much a key tile). CTA c works on the key tiles that begin in the stretch [c W, (c + 1) W) of the
+// line: whatever the lengths, every CTA gets the same work, and where a stretch ends inside a group its rows
 // are left as several partial results (running maximum, sum, unnormalised output), joined by the merge
 // kernel. A piece (c, group) has its partial rows at  2 * (rows of the groups before it) + c * ROWS:
 // pieces follow one another in c or in the group, and each takes at most min(2 rows, ROWS).
@@ -18,8 +18,6 @@
 
 namespace hc {
 
-constexpr int kOver = 1;  // virtual key tiles for the start of a group
-
 // Host constants of one call.
 struct LineShape {
   int T, n_seq, Hk, G, P;
@@ -27,6 +25,11 @@ struct LineShape {
   int nc;      // CTAs
   int nch;     // prefix chunks
   int dup;     // 2 where one piece may leave two partial results per row (two streams over the keys)
+};
+
+// What a group costs on the line: b to start it, a for each key tile.
+struct LineCost {
+  int a, b;
 };
 
 __host__ __device__ inline int ceil_div(int a, int b) { return (a + b - 1) / b; }
@@ -57,6 +60,16 @@ cudaError_t launch_prefix_mma(const PrefixArgs& a, const LineShape& s, int dtype
 // Whether a row tile of `rows` rows is taken by two streams over its key tiles, each with a result of its own
 // (hc_prefix_mma.cu): above that its halves, below it whole pieces go to one stream each.
 __host__ __device__ inline bool prefix_two_streams(int rows) { return rows > 64 && rows <= 128; }
+
+// fp32: alike. 16 bits, in units of about 0.55 us as measured on whole lines of one kind: tall row tiles
+// 2.7 us a key tile and 5.5 us to load Q and write the result, up to 64 rows 1.15 and 1.6 us.
+__device__ __forceinline__ LineCost line_cost(const LineShape& s, int rows) {
+  if (s.dup == 1) return {1, 1};
+  return rows > 128 ? LineCost{5, 10} : prefix_two_streams(rows) ? LineCost{3, 8} : LineCost{2, 3};
+}
+
+// The shortest stretch is >= every a: no CTA between a group's first and last is without a tile.
+__device__ __forceinline__ int min_stretch(const LineShape& s) { return s.dup == 1 ? 1 : 5; }
 
 struct Piece {
   bool own;         // suffix (own pages) or prefix
@@ -96,6 +109,7 @@ struct LineGeom {
   int R;              // query tokens of the call's sequences
   int tt;             // query tokens per row tile
   int nrt, ktp, ct;   // prefix row tiles, key tiles, key tiles per chunk
+  LineCost pre;       // of a prefix group
   int64_t head;       // length of one KV head's prefix groups
   int64_t vpre;       // length of all prefix groups
   __device__ LineGeom(const LineShape& s, int R_) {
@@ -104,11 +118,14 @@ struct LineGeom {
     nrt = ceil_div(R, tt);
     ktp = ceil_div(s.P, s.kt);
     ct = ktp > 0 ? ceil_div(ktp, s.nch) : 0;
-    head = ktp > 0 ? (int64_t)nrt * (ktp + s.nch * kOver) : 0;
+    pre = line_cost(s, min(R * s.G, s.rt));
+    head = ktp > 0 ? (int64_t)nrt * (ktp * pre.a + s.nch * pre.b) : 0;
     vpre = head * s.Hk;
   }
   __device__ int64_t seq_group(const LineShape& s, const SeqLens& q) const {  // one group of a sequence
-    return q.n > 0 && q.len > 0 ? ceil_div(q.len, s.kt) + kOver : 0;
+    if (q.n <= 0 || q.len <= 0) return 0;
+    const LineCost c = line_cost(s, min(q.n * s.G, s.rt));
+    return (int64_t)ceil_div(q.len, s.kt) * c.a + c.b;
   }
   __device__ int64_t seq_total(const LineShape& s, const SeqLens& q) const {
     return seq_group(s, q) * s.Hk * ceil_div(q.n, tt);
@@ -149,7 +166,7 @@ __device__ __forceinline__ Stretch line_setup(const PrefixArgs& a, const LineSha
   before += x - mine + g.vpre;
   total += g.vpre;
   Stretch r;
-  r.W = max((int64_t)line_div(total + s.nc - 1, s.nc), (int64_t)1);
+  r.W = max((int64_t)line_div(total + s.nc - 1, s.nc), (int64_t)min_stretch(s));
   r.v = min(c * r.W, total);
   r.v_end = min((c + 1) * r.W, total);
   if (c == 0 && tid == 0) hdr[0] = r.W;
@@ -185,9 +202,17 @@ struct LineWalk {
   bool own;
   SeqLens q;
   int len, nr;           // own pages: length of a group, row tiles of the sequence
+  LineCost cost;         // of the sequence's groups
+  // the key tiles of the group at v that begin in the stretch
+  __device__ __forceinline__ void clip(LineCost k, int tiles, int& lo, int& hi) const {
+    const int64_t s = cw - v - k.b, e = v_end - v - k.b;
+    lo = s <= 0 ? 0 : (int)min((s + k.a - 1) / k.a, (int64_t)tiles);
+    hi = e <= 0 ? 0 : (int)min((e + k.a - 1) / k.a, (int64_t)tiles);
+  }
   __device__ __forceinline__ void seq(const PrefixArgs& a, const LineShape& s, const LineGeom& g) {
     q = seq_lens(a, b);
     len = (int)g.seq_group(s, q);
+    cost = line_cost(s, min(q.n * s.G, s.rt));
     nr = len > 0 ? ceil_div(q.n, g.tt) : 0;
   }
   __device__ __forceinline__ LineWalk(const PrefixArgs& a, const LineShape& s, const LineGeom& g, const Stretch& st, int cta) {
@@ -201,11 +226,11 @@ struct LineWalk {
     if (v >= v_end) return;
     if (!own) {
       h = line_div(v, g.head);
-      const int rem = (int)(v - h * g.head), full = g.nrt * (g.ct + kOver);
-      j = min(rem / full, s.nch - 1);
-      const int n = min(g.ct, g.ktp - j * g.ct) + kOver;
-      r = (rem - j * full) / n;
-      v = h * g.head + (int64_t)j * full + (int64_t)r * n;
+      const int64_t rem = v - h * g.head, full = (int64_t)g.nrt * (g.ct * g.pre.a + g.pre.b);
+      j = min(line_div(rem, full), s.nch - 1);
+      const int64_t n = (int64_t)min(g.ct, g.ktp - j * g.ct) * g.pre.a + g.pre.b;
+      r = line_div(rem - j * full, n);
+      v = h * g.head + j * full + r * n;
     } else {
       seq(a, s, g);
       if (len > 0) {
@@ -220,7 +245,8 @@ struct LineWalk {
     while (v < v_end) {
       if (!own) {
         const int tiles = min(g.ct, g.ktp - j * g.ct);
-        const int lo = (int)max((int64_t)0, cw - v - kOver), hi = (int)min((int64_t)tiles, v_end - v - kOver);
+        int lo, hi;
+        clip(g.pre, tiles, lo, hi);
         p.own = false;
         p.b = 0;
         p.h = h;
@@ -231,7 +257,7 @@ struct LineWalk {
         p.kend = s.P;
         p.c0 = 0;
         p.row0 = s.dup * (((int64_t)h * s.nch + j) * s.T + p.tok0) * s.G + (int64_t)c * s.rt;
-        v += tiles + kOver;
+        v += (int64_t)tiles * g.pre.a + g.pre.b;
         if (++r == g.nrt) {
           r = 0;
           if (++j == s.nch) {
@@ -252,7 +278,8 @@ struct LineWalk {
         continue;
       }
       const int tok1 = min(q.n, (r + 1) * g.tt), keys = seq_keys(q, tok1), tiles = ceil_div(keys, s.kt);
-      const int lo = (int)max((int64_t)0, cw - v - kOver), hi = (int)min((int64_t)tiles, v_end - v - kOver);
+      int lo, hi;
+      clip(cost, tiles, lo, hi);
       p.own = true;
       p.b = b;
       p.h = h;

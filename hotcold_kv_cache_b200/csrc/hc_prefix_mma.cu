@@ -43,7 +43,7 @@ struct MmaSmem {
   static constexpr uint32_t pt = 16384;
   static constexpr uint32_t ring = 2 * qbuf;
   static constexpr uint32_t bars = ring + NB * tile;  // full[NB] empty[NB] s_full[2] p_ready[2] pv_done[2] q_ready[2] fin both
-  static constexpr uint32_t misc = (bars + 8 * (2 * NB + 10) + 15) & ~15u;  // tmem address, dead, armed, -, poison[3], turns[2]
+  static constexpr uint32_t misc = (bars + 8 * (2 * NB + 10) + 15) & ~15u;  // tmem address, dead, armed, q_here, poison[3], turns[2]
   static constexpr uint32_t red = misc + 48;  // per stream [4 warps][64 rows]; the setup's scan before that
   static constexpr uint32_t pieces = red + 2 * 4 * 64 * 4;           // the next pieces, and their barriers
   static constexpr uint32_t pbars = pieces + kPieces * sizeof(Piece);  // full[kPieces] empty[kPieces]
@@ -134,12 +134,11 @@ __device__ __forceinline__ void wait_full(uint64_t* full, uint32_t n, volatile u
                                           int32_t* status) {
   for (int i = 0; *armed <= n; ++i) {
     if (*dead) return;
-    if (i == kMaxPolls) {
+    if (i == 16 * kMaxPolls) {
       *dead = 1;
       if (status) atomicOr(status, HC_DEV_TIMEOUT);
       return;
     }
-    __nanosleep(64);
   }
   wait_bar(&full[n % NB], (n / NB) & 1, dead, status);
 }
@@ -173,7 +172,8 @@ __device__ __forceinline__ float redux_max(float x) {
 // Stream x's turn for its tall tile number n: the first stream goes when the other has issued all S tiles
 // before n, the second when the first has issued S tile n.
 __device__ __forceinline__ void wait_turn(volatile uint32_t* turns, int x, uint32_t n, volatile int* dead) {
-  for (int i = 0; turns[x ^ 1] < n + x && !*dead && i < kMaxPolls; ++i) __nanosleep(20);
+  for (int i = 0; turns[x ^ 1] < n + x && !*dead && i < 16 * kMaxPolls; ++i) {
+  }
 }
 // Shared-memory descriptors from their low word's address (see umma_desc_k_sw128, umma_desc_mn_sw128).
 __device__ __forceinline__ uint64_t desc_k(uint32_t addr16) {
@@ -600,7 +600,8 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
   volatile int* dead = reinterpret_cast<volatile int*>(smem + SM::misc + 4);
   volatile uint32_t* armed = reinterpret_cast<volatile uint32_t*>(smem + SM::misc + 8);  // ring positions armed
   uint64_t* both = fin + 1;
-  volatile uint32_t* turns = armed + 5;  // per stream: S tiles of tall row tiles issued
+  volatile uint32_t* q_here = armed + 1;  // the first Q rows have arrived
+  volatile uint32_t* turns = armed + 5;   // per stream: S tiles of tall row tiles issued
   int* poison = reinterpret_cast<int*>(smem + SM::misc + 16);  // a hidden value was not finite: per stream, and both halves'
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, G = ls.G;
   PieceRing ring{reinterpret_cast<const Piece*>(smem + SM::pieces), reinterpret_cast<uint64_t*>(smem + SM::pbars),
@@ -625,7 +626,7 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     mbar_init(both, 8);
     fence_mbar_init();
     *dead = 0;
-    *armed = 0;
+    *armed = *q_here = 0;
     poison[0] = poison[1] = poison[2] = 0;
     turns[0] = turns[1] = 0;
     prefetch_tensormap(&maps.kp);
@@ -668,6 +669,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
           }
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv, ++n) {
+            // the first Q rows do not queue behind a ring full of tiles
+            if (n == 2)
+              for (int i = 0; !*q_here && !*dead && i < kMaxPolls; ++i) __nanosleep(20);
             const uint32_t b = n % NB;
             wait_bar(&empty[b], ((n / NB) & 1) ^ 1, dead, a.status);
             unsigned char* dst = smem + SM::ring + b * SM::tile;
@@ -801,27 +805,27 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         if (prefix_two_streams(tq.rows) && r < tq.rows) ml[q.row0 + tq.rows + r] = make_float2(kNegInf, 0.f);
       }
     };
-    // its Q rows: 16 bytes a thread at a time, all loads in flight, then into the swizzled K-major layout
-    constexpr int CPR = D / 8, QB = 128 * CPR / 128;
-    uint4 u[QB];
-    auto load_q = [&]() {
-      const int total = tq.nr * CPR;
+    // its Q rows: a thread takes one 16-byte column of every RS-th row (a whole number of tokens apart, since
+    // the group divides RS), all loads in flight, then into the swizzled K-major layout
+    constexpr int CPR = D / 8, RS = 128 / CPR, QB = 128 / RS;
+    const int qc = r % CPR, qr = r / CPR;
+    auto load_q = [&](uint4* u) {
+      const int row = tq.row_at + qr;
+      const T* src = reinterpret_cast<const T*>(a.q) + (int64_t)(q.tok0 + (row >> lg)) * a.q_st +
+                     (int64_t)(q.h * G + (row & (G - 1))) * a.q_sh + qc * 8;
+      const int64_t step = (int64_t)(RS >> lg) * a.q_st;
 #pragma unroll
       for (int j = 0; j < QB; ++j) {
-        const int k = r + j * 128, row = tq.row_at + k / CPR;
-        if (k < total)
-          u[j] = reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (int64_t)(q.tok0 + (row >> lg)) * a.q_st +
-                                                (int64_t)(q.h * G + (row & (G - 1))) * a.q_sh)[k % CPR];
+        u[j] = qr + j * RS < tq.nr ? *reinterpret_cast<const uint4*>(src) : make_uint4(0u, 0u, 0u, 0u);
+        src += step;
       }
     };
-    auto store_q = [&]() {
-      const int total = tq.nr * CPR;
+    auto store_q = [&](const uint4* u) {
       const uint32_t plane = tq.mode == kTransposed ? t_cols(tq.nr) * 128u : 16384u;
+      unsigned char* dst = sQ + (qc >> 3) * plane + qr * 128 + (((qc & 7) ^ (qr & 7)) << 4);
 #pragma unroll
-      for (int j = 0; j < QB; ++j) {
-        const int k = r + j * 128, rr = k / CPR, c = k % CPR;
-        if (k < total) *reinterpret_cast<uint4*>(sQ + (c >> 3) * plane + rr * 128 + (((c & 7) ^ (rr & 7)) << 4)) = u[j];
-      }
+      for (int j = 0; j < QB; ++j)
+        if (qr + j * RS < tq.nr) *reinterpret_cast<uint4*>(dst + j * RS * 128) = u[j];
       fence_proxy_async_smem();
     };
     auto q_arrive = [&]() {
@@ -830,8 +834,10 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     };
     bool have = advance();
     if (have) {
-      load_q();
-      store_q();
+      uint4 u[QB];
+      load_q(u);
+      store_q(u);
+      if (r == 0) *q_here = 1;
       q_arrive();
     }
     while (have) {
@@ -845,17 +851,33 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       float m = kNegInf, l = 0.f;
       bool any = false;
       const bool tr = t.mode == kTransposed;
-      if (!tr) rows_tiles<DT, D>(f, nt, m, l, any);
-      else if (t.nr <= 8) any = cols_tiles<DT, D, 8>(f, nt, ml);
-      else if (t.nr <= 16) any = cols_tiles<DT, D, 16>(f, nt, ml);
-      else if (t.nr <= 32) any = cols_tiles<DT, D, 32>(f, nt, ml);
-      else any = cols_tiles<DT, D, 64>(f, nt, ml);
-      have = advance();
-      if (have) load_q();
+      // the next piece is fetched and its Q rows are under way during this one's tiles, where a thread has
+      // registers for them
+      uint4 u[QB];
+      auto fetch = [&]() {
+        have = advance();
+        if (have) load_q(u);
+      };
+      if (!tr) {
+        rows_tiles<DT, D>(f, nt, m, l, any);
+        fetch();
+      } else if (t.nr <= 8) {
+        fetch();
+        any = cols_tiles<DT, D, 8>(f, nt, ml);
+      } else if (t.nr <= 16) {
+        fetch();
+        any = cols_tiles<DT, D, 16>(f, nt, ml);
+      } else if (t.nr <= 32) {
+        fetch();
+        any = cols_tiles<DT, D, 32>(f, nt, ml);
+      } else {
+        any = cols_tiles<DT, D, 64>(f, nt, ml);
+        fetch();
+      }
       wait_bar(&pv_done[x], (nt - 1) & 1, dead, a.status);
       tc_fence_after();
       if (have) {
-        store_q();
+        store_q(u);
         q_arrive();
       }
       if (!tr) rows_out<DT, D>(f, m, l, any, ml, part);

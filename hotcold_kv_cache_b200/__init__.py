@@ -37,7 +37,8 @@ def __getattr__(name):
         return triton_evict_attention_forward
     if name in ("PagePlan", "plan_pages", "release_pages", "append_pages", "shared_prefix_attention"):
         from . import prefix
-        return getattr(prefix, name)
+        globals()[name] = getattr(prefix, name)  # found without this function from now on
+        return globals()[name]
     if name == "KVController":
         from .controller import KVController
         return KVController

@@ -79,6 +79,7 @@ struct PagePlanArgs {
   int64_t* positions;
   int32_t* status;
   int n_seq, page_size, max_blocks, n_pages, n_tokens, base_pos;
+  int in_place, only_commit;  // set by launch_plan_pages
 };
 struct PageAppendArgs {
   const void *q, *k, *v;

@@ -8,9 +8,10 @@
 //   block_table[b][have_b + i] = free[n_free - 1 - first_b - i],  i < need_b
 //   token t of sequence b (cu_b <= t < cu_{b+1}) sits at p = len_b + t - cu_b, slot = page * ps + p % ps
 // It is bound by latency (a launch, two dependent loads, one block scan): 12 bytes a sequence and 20 a
-// token. Every CTA scans the lengths of all sequences for itself (at most 4096, 8 a thread), so the
-// tokens spread over a cluster of up to 8 CTAs without a second launch; a cluster, because lens and
-// n_free may be updated in place, which the first CTA does once all have read them.
+// token. Every CTA scans the lengths of all sequences for itself (at most 4096, 8 a thread), so the tokens
+// spread over CTAs without a second launch. lens and n_free may be updated in place, which has to come
+// after every CTA has read them: up to 8 CTAs are a cluster and meet before the first one does it; the
+// slot maps of whole prompts take as many CTAs as they fill, and a second launch of one CTA commits.
 
 #include "hc_internal.cuh"
 
@@ -80,38 +81,42 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(PagePlanArgs a
     if (i >= per || b >= a.n_seq) continue;
     s_cu[b] = cu;
     s_first[b] = first;
-    if (rank == 0) a.cu_new[b] = cu;
+    if (rank == 0 && !a.only_commit) a.cu_new[b] = cu;
     if (ok) {
       cu += add[i];
       first += (int)(((long long)len[i] + add[i] + pm) >> sh) - (int)(((long long)len[i] + pm) >> sh);
     }
   }
   if (tid == 0) {
-    if (rank == 0) a.cu_new[a.n_seq] = total;
+    if (rank == 0 && !a.only_commit) a.cu_new[a.n_seq] = total;
     if (rank == 0 && bits && a.status) atomicOr(a.status, bits);
   }
   __syncthreads();
   const int step = nct * kPlanThreads;
-  for (int f = rank * kPlanThreads + tid; f < fresh; f += step) {
-    const int b = last_not_above(s_first, a.n_seq, f);
-    a.block_table[(size_t)b * a.max_blocks + ((a.lens[b] + pm) >> sh) + (f - s_first[b])] = a.free_pages[n_free - 1 - f];
-  }
-  for (int t = rank * kPlanThreads + tid; t < a.n_tokens; t += step) {
-    int64_t slot = -1, pos = -1;
-    int b = -1;
-    if (t < total) {
-      b = last_not_above(s_cu, a.n_seq, t);
-      const int len0 = a.lens[b], p = len0 + (t - s_cu[b]), j = p >> sh, have = (len0 + pm) >> sh;
-      const int page = j < have ? a.block_table[(size_t)b * a.max_blocks + j] : a.free_pages[n_free - 1 - s_first[b] - (j - have)];
-      if (page >= 0 && page < a.n_pages) slot = ((int64_t)page << sh) + (p & pm);
-      else if (a.status) atomicOr(a.status, HC_DEV_INDEX);
-      pos = (int64_t)a.base_pos + p;
+  if (!a.only_commit) {
+    for (int f = rank * kPlanThreads + tid; f < fresh; f += step) {
+      const int b = last_not_above(s_first, a.n_seq, f);
+      a.block_table[(size_t)b * a.max_blocks + ((a.lens[b] + pm) >> sh) + (f - s_first[b])] = a.free_pages[n_free - 1 - f];
     }
-    a.slots[t] = slot;
-    a.seq_ids[t] = b;
-    a.positions[t] = pos;
+#pragma unroll 2
+    for (int t = rank * kPlanThreads + tid; t < a.n_tokens; t += step) {
+      int64_t slot = -1, pos = -1;
+      int b = -1;
+      if (t < total) {
+        b = last_not_above(s_cu, a.n_seq, t);
+        const int len0 = a.lens[b], p = len0 + (t - s_cu[b]), j = p >> sh, have = (len0 + pm) >> sh;
+        const int page = j < have ? a.block_table[(size_t)b * a.max_blocks + j] : a.free_pages[n_free - 1 - s_first[b] - (j - have)];
+        if (page >= 0 && page < a.n_pages) slot = ((int64_t)page << sh) + (p & pm);
+        else if (a.status) atomicOr(a.status, HC_DEV_INDEX);
+        pos = (int64_t)a.base_pos + p;
+      }
+      a.slots[t] = slot;
+      a.seq_ids[t] = b;
+      a.positions[t] = pos;
+    }
   }
-  if (nct > 1) cluster_sync_all();  // every CTA has read lens and n_free: they may be updated in place
+  if (!a.lens_out) return;  // committed by another launch
+  if (a.in_place && nct > 1) cluster_sync_all();  // every CTA has read lens and n_free
   else __syncthreads();
   if (rank == 0) {
 #pragma unroll
@@ -176,10 +181,23 @@ __global__ void __launch_bounds__(kPlanThreads) release_pages_kernel(PagePlanArg
   if (tid == 0) *a.n_free_out = n_free + total;
 }
 
-cudaError_t launch_plan_pages(const PagePlanArgs& a, cudaStream_t stream) {
-  // one CTA for what a CTA does in a few rounds, up to 8 for the slot maps of whole prompts
+// One B200, a step of 64 tokens 5 us; 147 thousand tokens of 256 prompts see the token loop's width: 51 us on
+// 8 CTAs, PLAN_GRID_US on as many as a thousand tokens each fill (2.9 MB written).
+cudaError_t launch_plan_pages(const PagePlanArgs& args, cudaStream_t stream) {
+  PagePlanArgs a = args;
+  a.in_place = a.lens == a.lens_out || a.n_free == a.n_free_out;
+  const int want = (int)(((int64_t)a.n_tokens + kPlanThreads - 1) / kPlanThreads);
+  if (want > 16) {
+    const int ctas = want / 2 < 296 ? want / 2 : 296;
+    if (a.in_place) a.lens_out = nullptr;
+    cudaError_t e = launch_pdl(plan_pages_kernel, dim3((unsigned)ctas), dim3(kPlanThreads), 0, stream, a);
+    if (e != cudaSuccess || !a.in_place) return e;
+    a.lens_out = args.lens_out;
+    a.only_commit = 1;
+    return launch_pdl(plan_pages_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a);
+  }
   int ctas = 1;
-  while (ctas < 8 && (int64_t)ctas * kPlanThreads * 4 < a.n_tokens) ctas *= 2;
+  while (ctas < 8 && ctas < want) ctas *= 2;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;

@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kSimtThreads, 2) prefix_simt_kernel(PrefixArgs
 // A row with no attended key at all is 0 with a log-sum of -inf. Bound by the partial results it reads
 // (from L2) and, for a decode step, by its launch and three dependent reads.
 // ----------------------------------------------------------------------------------------
-constexpr int kMergeThreads = 128;
+constexpr int kMergeThreads = 256;
 constexpr int kMaxCtas = 448;     // CTAs a call's work is divided among
 constexpr int kMergeList = 512;   // >= partial results of a row: one per CTA and one more per group of the row (17)
 
@@ -244,21 +244,23 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(PrefixArgs 
   using T = typename E::T;
   __shared__ int64_t list[kMergeList];
   __shared__ float wts[kMergeList * 8];
-  __shared__ float s_ml[16];
-  __shared__ int s_n[2], s_b, s_geo[4];
+  __shared__ float4 sum[kMergeThreads];
+  __shared__ float s_ml[8];
+  __shared__ int s_b, s_geo[4], s_lo[17], s_at[18], s_sec[17];
+  __shared__ int64_t s_row[17];
   const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  pdl_wait();
-  const int R = min(a.T, max(a.cu_new[s.n_seq], 0));
-  if (t >= R) return;  // rows behind the last sequence are left as they were
-  const LineGeom g(s, R);
-  const int64_t W = hdr[0];
   if (tid == 0) s_b = -1;
+  pdl_wait();
+  const int64_t W = hdr[0];
+  const int R = min(a.T, max(a.cu_new[s.n_seq], 0));
   __syncthreads();
   for (int b = tid; b < s.n_seq; b += kMergeThreads)
     if (a.cu_new[b] <= t && t < a.cu_new[b + 1]) s_b = b;
+  if (t >= R) return;  // rows behind the last sequence are left as they were
+  const LineGeom g(s, R);
   __syncthreads();
-  // the blocks of partial rows over these rows, in a fixed order: lane j < nch the prefix chunk j, lane nch
-  // the own pages; where a CTA ran two streams over the keys, both of its blocks
+  // the blocks of partial rows over these rows, in a fixed order: segment j < nch the prefix chunk j, segment
+  // nch the own pages; where a CTA ran two streams over the keys, both of its blocks
   if (warp == 0) {
     int64_t row = 0;
     int lo = 0, hi = -1, rows = 0, q0 = 0;
@@ -292,37 +294,39 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(PrefixArgs 
       const int y = __shfl_up_sync(0xffffffffu, at, o);
       if (lane >= o) at += y;
     }
-    const int before = __shfl_up_sync(0xffffffffu, at, 1);
-    if (lane == 0) {
-      s_geo[0] = n_blk;  // rows of a prefix block, and the first of these rows in it
-      s_geo[1] = q0 - blk;
+    if (lane <= s.nch) {
+      s_lo[lane] = lo;
+      s_row[lane] = row + blk;
+      s_sec[lane] = second ? rows : 0;
+      s_at[lane + 1] = min(at, kMergeList);
     }
-    if (lane == s.nch) {
-      s_geo[2] = n_blk;
-      s_geo[3] = q0 - blk;
-      s_n[0] = min(before, kMergeList);  // prefix blocks, then those of the own pages
-      s_n[1] = min(at, kMergeList);
+    if (lane == 0 || lane == s.nch) {  // rows of a block, and the first of these rows in it: prefix, own pages
+      s_geo[lane ? 2 : 0] = n_blk;
+      s_geo[lane ? 3 : 1] = q0 - blk;
     }
-    at -= mine;
-    for (int c = lo; c <= hi; ++c) {
-      const int64_t base = row + (int64_t)c * s.rt + blk;
-      if (at < kMergeList) list[at] = base;
-      ++at;
-      if (second) {
-        if (at < kMergeList) list[at] = base + rows;
-        ++at;
-      }
-    }
+    if (lane == 0) s_at[0] = 0;
   }
   __syncthreads();
-  const int np = s_n[0], n = s_n[1];
+  const int np = s_at[s.nch], n = s_at[s.nch + 1];
   for (int gq = warp; gq < s.G; gq += kMergeThreads / 32) {
+    // a lane's first block stays in registers; the maximum needs the others once more
     float M = kNegInf, L = 0.f;
-    for (int x = lane; x < n; x += 32) M = fmaxf(M, __ldcg(&ml[list[x] + (x < np ? s_geo[1] : s_geo[3]) + gq]).x);
+    float2 z0 = make_float2(kNegInf, 0.f);
+    auto load = [&](int x) {
+      int j = 0;
+      while (x >= s_at[j + 1]) ++j;
+      const int i = x - s_at[j], sec = s_sec[j];
+      const int64_t base = s_row[j] + (int64_t)(s_lo[j] + (sec ? i >> 1 : i)) * s.rt + (sec && (i & 1) ? sec : 0);
+      if (gq == 0) list[x] = base;
+      return __ldcg(&ml[base + (j < s.nch ? s_geo[1] : s_geo[3]) + gq]);
+    };
+    if (lane < n) z0 = load(lane);
+    M = z0.x;
+    for (int x = lane + 32; x < n; x += 32) M = fmaxf(M, load(x).x);
     M = warp_max(M);
     const float ref = M == kNegInf ? 0.f : M;
     for (int x = lane; x < n; x += 32) {
-      const float2 z = __ldcg(&ml[list[x] + (x < np ? s_geo[1] : s_geo[3]) + gq]);
+      const float2 z = x < 32 ? z0 : load(x);
       const float w = ex2(z.x - ref);
       wts[x * s.G + gq] = w;
       L = fmaf(w, z.y, L);
@@ -334,24 +338,41 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(PrefixArgs 
     }
   }
   __syncthreads();
-  for (int k = tid; k < s.G * (D / 4); k += kMergeThreads) {
+  // columns of 16 bytes x rows, and where there are fewer of them than threads the blocks in as many shares
+  const int items = s.G * (D / 4), shares = items < kMergeThreads ? kMergeThreads / items : 1;
+  for (int k0 = 0; k0 < items; k0 += kMergeThreads) {
+    const int k = k0 + tid % items, share = tid / items;
     const int gq = k & (s.G - 1), c4 = k / s.G;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](int x, const float* src) {
-      const float w = wts[x * s.G + gq];
-      const float4 y = __ldcg(reinterpret_cast<const float4*>(src));
-      if (w != 0.f) {  // a block without a key may not have been written
-        o.x = fmaf(w, y.x, o.x);
-        o.y = fmaf(w, y.y, o.y);
-        o.z = fmaf(w, y.z, o.z);
-        o.w = fmaf(w, y.w, o.w);
-      }
-    };
     const size_t off_p = ((size_t)c4 * s_geo[0] + s_geo[1] + gq) * 4, off_s = ((size_t)c4 * s_geo[2] + s_geo[3] + gq) * 4;
-#pragma unroll 4
-    for (int x = 0; x < np; ++x) add(x, part + (size_t)list[x] * D + off_p);
-#pragma unroll 4
-    for (int x = np; x < n; ++x) add(x, part + (size_t)list[x] * D + off_s);
+    for (int x0 = share; x0 < n; x0 += 8 * shares) {
+      float4 y[8];
+      float w[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int x = x0 + u * shares;
+        w[u] = x < n ? wts[x * s.G + gq] : 0.f;
+        // a block without a key may not have been written
+        y[u] = w[u] != 0.f ? __ldcg(reinterpret_cast<const float4*>(part + (size_t)list[x] * D + (x < np ? off_p : off_s)))
+                           : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        o.x = fmaf(w[u], y[u].x, o.x);
+        o.y = fmaf(w[u], y[u].y, o.y);
+        o.z = fmaf(w[u], y[u].z, o.z);
+        o.w = fmaf(w[u], y[u].w, o.w);
+      }
+    }
+    if (shares > 1) {
+      sum[tid] = o;
+      __syncthreads();
+      if (share > 0) break;
+      for (int z = 1; z < shares; ++z) {
+        const float4 y = sum[z * items + k];
+        o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
+      }
+    }
     const float L = s_ml[gq], inv = L == 0.f ? 0.f : 1.f / L;
     alignas(16) T r[4];
     r[0] = E::from_f(L == 0.f ? 0.f : o.x * inv);

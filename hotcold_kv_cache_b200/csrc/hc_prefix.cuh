@@ -100,9 +100,11 @@ __device__ __forceinline__ int seq_keys(const SeqLens& s, int tok1) {  // keys s
   return min(max(s.len - s.n + tok1, 0), s.len);
 }
 
-// Quotient of line positions: 64-bit division only where 32 bits do not hold them.
+// Quotient of line positions: 64-bit division, out of the way, only where 32 bits do not hold them (a kernel
+// starts with cold instruction caches, and its first microseconds are fetches of what it runs through).
+static __device__ __noinline__ int line_div64(int64_t x, int64_t y) { return (int)(x / y); }
 __device__ __forceinline__ int line_div(int64_t x, int64_t y) {
-  return (x | y) >> 32 ? (int)(x / y) : (int)((uint32_t)x / (uint32_t)y);
+  return (x | y) >> 32 ? line_div64(x, y) : (int)((uint32_t)x / (uint32_t)y);
 }
 
 struct LineGeom {
@@ -206,8 +208,9 @@ struct LineWalk {
   // the key tiles of the group at v that begin in the stretch
   __device__ __forceinline__ void clip(LineCost k, int tiles, int& lo, int& hi) const {
     const int64_t s = cw - v - k.b, e = v_end - v - k.b;
-    lo = s <= 0 ? 0 : (int)min((s + k.a - 1) / k.a, (int64_t)tiles);
-    hi = e <= 0 ? 0 : (int)min((e + k.a - 1) / k.a, (int64_t)tiles);
+    const int64_t all = (int64_t)tiles * k.a;  // beyond it every tile counts
+    lo = s <= 0 ? 0 : s >= all ? tiles : line_div(s + k.a - 1, k.a);
+    hi = e <= 0 ? 0 : e >= all ? tiles : line_div(e + k.a - 1, k.a);
   }
   __device__ __forceinline__ void seq(const PrefixArgs& a, const LineShape& s, const LineGeom& g) {
     q = seq_lens(a, b);

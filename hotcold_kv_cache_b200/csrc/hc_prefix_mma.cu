@@ -304,22 +304,23 @@ __device__ __forceinline__ bool clean_v(const Soft& f, int i, int k0, bool maske
     for (int c = 0; c < SM::PL * 8; ++c)
       *reinterpret_cast<uint4*>(sV + (c >> 3) * 16384 + (((c & 7) ^ rot) << 4)) = make_uint4(0u, 0u, 0u, 0u);
   } else if (scan && key > f.p.c0 && (!half || f.x == 0)) {
+    // a 16-bit value is not finite when its exponent bits are all ones, i.e. carry into the top bit
+    constexpr uint32_t kExp = DT == HC_F16 ? 0x7c007c00u : 0x7f807f80u, kOne = DT == HC_F16 ? 0x04000400u : 0x00800080u;
     bool odd = false;
-#pragma unroll 2
+#pragma unroll 4
     for (int c = 0; c < SM::PL * 8; ++c) {
       uint4* at = reinterpret_cast<uint4*>(sV + (c >> 3) * 16384 + (((c & 7) ^ rot) << 4));
       const uint4 u = *at;
-      float v[8];
-      unpack16<DT>(u, v);
-      bool bad = false;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) bad |= !isfinite(v[e]);
-      if (bad) {
+      if ((((u.x & kExp) + kOne) | ((u.y & kExp) + kOne) | ((u.z & kExp) + kOne) | ((u.w & kExp) + kOne)) & 0x80008000u) {
         odd = true;
-        alignas(16) T z[8];
+        const uint32_t y[4] = {u.x, u.y, u.z, u.w};
+        uint32_t z[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) z[e] = Elem<DT>::from_f(isfinite(v[e]) ? v[e] : 0.f);
-        *at = *reinterpret_cast<uint4*>(z);
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t bad = (((y[e] & kExp) + kOne) & 0x80008000u) >> 15;  // 1 in each half that is not finite
+          z[e] = y[e] & ~(bad * 0xffffu);
+        }
+        *at = make_uint4(z[0], z[1], z[2], z[3]);
       }
     }
     if (odd) atomicOr(f.poison, 1);
@@ -510,6 +511,10 @@ __device__ __forceinline__ bool cols_tiles(const Soft& f, uint32_t& nt, float2* 
     }
     t0 *= f.sc;
     t1 *= f.sc;
+    if (i > 0) {  // the last tile's O += P V: its P^T is written over now, and O may be rescaled
+      wait_bar(f.pv_done, (nt - 1) & 1, f.dead, f.a.status);
+      tc_fence_after();
+    }
     const bool up = (lane < nr && t0 > m0 + kLazy) || (N > 32 && 32 + lane < nr && t1 > m1 + kLazy);
     if (__any_sync(0xffffffffu, up)) {
       const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
@@ -716,7 +721,9 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
             const uint32_t nk = base + 2 * i, nv = nk + 1, bk = nk % NB, bv = nv % NB;
             const uint32_t dk = dr + bk * (SM::tile >> 4), dv = dr + bv * (SM::tile >> 4);
             wait_full<NB>(full, nk, armed, dead, a.status);
-            if (nt > 0) wait_bar(&pv_done[x], (nt - 1) & 1, dead, a.status);  // P of the last tile has been read
+            // P of the last tile, in the columns of S, has been read; transposed, the scores of the last tile were
+            // in registers once P^T was ready
+            if (!tr && i > t.first) wait_bar(&pv_done[x], (nt - 1) & 1, dead, a.status);
             if (half && i == 0) wait_turn(turns, x, tall, dead);
             tc_fence_after();
             if (leader) {

@@ -34,6 +34,8 @@ class PagePlan(NamedTuple):
 
 
 _FN: dict = {}
+_SCRATCH_BYTES: dict = {}
+_I32, _I64 = torch.int32, torch.int64
 
 
 def _call(name: str, device, *args):
@@ -52,14 +54,15 @@ def _call(name: str, device, *args):
 
 def _check(name: str, t: torch.Tensor, dtype, shape, device):
     """A contiguous CUDA tensor of this dtype, shape and device."""
+    if t.dtype is dtype and t.shape == shape and t.device == device and t.is_contiguous():
+        return
     if t.dtype is not dtype:
         raise TypeError(f"{name} must be {dtype}, not {t.dtype}")
     if t.device != device:
         raise ValueError(f"{name} is on {t.device}, not on {device}")
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, not {tuple(t.shape)}")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
+    raise ValueError(f"{name} must be contiguous")
 
 
 def _cuda(name: str, t: torch.Tensor):
@@ -84,7 +87,7 @@ def plan_pages(lens, new_lens, block_table, free_pages, n_free, page_size: int, 
     HC_DEV_INDEX."""
     dev = _cuda("lens", lens)
     n_seq, max_blocks = block_table.shape
-    i32, i64 = torch.int32, torch.int64
+    i32, i64 = _I32, _I64
     n_tokens = int(n_tokens)
     _check("lens", lens, i32, (n_seq,), dev)
     _check("new_lens", new_lens, i32, (n_seq,), dev)
@@ -119,7 +122,7 @@ def release_pages(lens, keep_lens, block_table, free_pages, n_free, page_size: i
     given, gets HC_DEV_INDEX or HC_DEV_CAPACITY."""
     dev = _cuda("lens", lens)
     n_seq, max_blocks = block_table.shape
-    i32 = torch.int32
+    i32 = _I32
     _check("lens", lens, i32, (n_seq,), dev)
     _check("keep_lens", keep_lens, i32, (n_seq,), dev)
     _check("block_table", block_table, i32, (n_seq, max_blocks), dev)
@@ -218,7 +221,7 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k_pages, v_pages, block_table
     Hk = k_pages.shape[1]
     n_pages, page_size = _pools(k_pages, v_pages, Hk, D, dtype, dev)
     n_seq, max_blocks = block_table.shape
-    i32 = torch.int32
+    i32 = _I32
     _check("block_table", block_table, i32, (n_seq, max_blocks), dev)
     _check("lens", lens, i32, (n_seq,), dev)
     _check("cu_new", cu_new, i32, (n_seq + 1,), dev)
@@ -245,7 +248,13 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k_pages, v_pages, block_table
     if status is not None:
         _check("status", status, i32, (1,), dev)
     if T > 0:
-        nbytes = _lib.size("hc_shared_prefix_attention_scratch_bytes", code, T, n_seq, Hq, Hk, D, P)
+        key = (dev.index, code, T, n_seq, Hq, Hk, D, P)
+        nbytes = _SCRATCH_BYTES.get(key)
+        if nbytes is None:
+            with torch.cuda.device(dev):  # the work is divided among this device's multiprocessors
+                nbytes = _lib.size("hc_shared_prefix_attention_scratch_bytes", code, T, n_seq, Hq, Hk, D, P)
+            if len(_SCRATCH_BYTES) < 4096:
+                _SCRATCH_BYTES[key] = nbytes
         # this call's own: two streams, or two captured graphs, never share it
         scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
         q_st, q_sh, _ = q.stride()

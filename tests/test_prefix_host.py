@@ -39,7 +39,7 @@ def attend_args(**kw):
     (dict(P=-1), b"prefix"), (dict(page=24), b"page_size"), (dict(page=8), b"page_size"), (dict(page=512), b"page_size"),
     (dict(blocks=0), b"max_blocks"), (dict(blocks=1 << 28), b"max_blocks"), (dict(pages=0), b"n_pages"),
     (dict(q=None), b"NULL"), (dict(pk=None), b"prefix"), (dict(scale=0.0), b"scaling"), (dict(scale=float("nan")), b"scaling"),
-    (dict(q=4098), b"aligned"), (dict(q_st=1001), b"aligned"), (dict(pv_st=1001), b"aligned"), (dict(kp=4104), b"aligned"),
+    (dict(q=4098), b"aligned"), (dict(T=2, q_st=1001), b"aligned"), (dict(pv_st=1001), b"aligned"), (dict(kp=4104), b"aligned"),
     (dict(), b"scratch")])
 def test_attention_refusals_launch_nothing(kw, word):
     lib = _lib.load()

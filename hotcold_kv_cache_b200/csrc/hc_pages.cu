@@ -32,6 +32,32 @@ __device__ __forceinline__ int last_not_above(const int* s, int n, int x) {
   return lo;
 }
 
+// Exclusive sums over the block of two counts per thread, and their totals. 64 bits: the totals of refused
+// lengths are looked at too. `sh` takes 2 * kPlanThreads / 32 values. (64-bit atomics on one shared word
+// took 15 us for 256 threads.)
+__device__ __forceinline__ void scan_pair(int64_t x, int64_t y, int64_t* sh, int64_t& bx, int64_t& by, int64_t& tx, int64_t& ty) {
+  constexpr int NW = kPlanThreads / 32;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  bx = x;
+  by = y;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int64_t p = __shfl_up_sync(0xffffffffu, bx, o), q = __shfl_up_sync(0xffffffffu, by, o);
+    if (lane >= o) bx += p, by += q;
+  }
+  if (lane == 31) sh[warp] = bx, sh[NW + warp] = by;
+  __syncthreads();
+  bx -= x;
+  by -= y;
+  tx = ty = 0;
+#pragma unroll
+  for (int w = 0; w < NW; ++w) {
+    if (w == warp) bx += tx, by += ty;
+    tx += sh[w];
+    ty += sh[NW + w];
+  }
+}
+
 __device__ __forceinline__ void cluster_sync_all() {
   __syncthreads();
   cluster_arrive();
@@ -40,14 +66,11 @@ __device__ __forceinline__ void cluster_sync_all() {
 
 __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(PagePlanArgs a) {
   __shared__ int s_cu[kPlanMaxSeq], s_first[kPlanMaxSeq];
-  __shared__ int s_scan[kPlanThreads / 32 + 1];
-  __shared__ long long s_tot[2];
+  __shared__ int64_t s_scan[2 * kPlanThreads / 32];
   pdl_wait();
   const int tid = threadIdx.x, rank = blockIdx.x, nct = gridDim.x;
   const int sh = __ffs(a.page_size) - 1, pm = a.page_size - 1;
   const long long cap = (long long)a.max_blocks << sh;
-  if (tid < 2) s_tot[tid] = 0;
-  __syncthreads();
   const int n_free = *a.n_free;
   const int per = (a.n_seq + kPlanThreads - 1) / kPlanThreads;
   int len[kPlanPer], add[kPlanPer];
@@ -66,15 +89,13 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(PagePlanArgs a
       np += (int)(((long long)len[i] + add[i] + pm) >> sh) - (int)(((long long)len[i] + pm) >> sh);
     }
   }
-  if (nn) atomicAdd(reinterpret_cast<unsigned long long*>(&s_tot[0]), (unsigned long long)nn);
-  if (np) atomicAdd(reinterpret_cast<unsigned long long*>(&s_tot[1]), (unsigned long long)np);
+  int64_t cu0, first0, all_new, all_fresh;
+  scan_pair(nn, np, s_scan, cu0, first0, all_new, all_fresh);
   const int bad_index = __syncthreads_or(bits & HC_DEV_INDEX), bad_cap = __syncthreads_or(bits & HC_DEV_CAPACITY);
-  bits = (bad_index ? HC_DEV_INDEX : 0) | (bad_cap || s_tot[0] > a.n_tokens || s_tot[1] > n_free ? HC_DEV_CAPACITY : 0);
+  bits = (bad_index ? HC_DEV_INDEX : 0) | (bad_cap || all_new > a.n_tokens || all_fresh > n_free ? HC_DEV_CAPACITY : 0);
   const bool ok = bits == 0;
-  const int total = ok ? (int)s_tot[0] : 0, fresh = ok ? (int)s_tot[1] : 0;
-  // exclusive scans of the new tokens and the fresh pages; both totals fit an int here
-  int dummy, cu = block_exclusive_scan(ok ? (int)nn : 0, s_scan, dummy);
-  int first = block_exclusive_scan(ok ? (int)np : 0, s_scan, dummy);
+  const int total = ok ? (int)all_new : 0, fresh = ok ? (int)all_fresh : 0;
+  int cu = ok ? (int)cu0 : 0, first = ok ? (int)first0 : 0;
 #pragma unroll
   for (int i = 0; i < kPlanPer; ++i) {
     const int b = tid * per + i;
@@ -132,14 +153,11 @@ __global__ void __launch_bounds__(kPlanThreads) plan_pages_kernel(PagePlanArgs a
 // the order plan_pages_kernel takes them, so that taking a step back restores the stack as it was.
 __global__ void __launch_bounds__(kPlanThreads) release_pages_kernel(PagePlanArgs a) {
   __shared__ int s_first[kPlanMaxSeq], s_have[kPlanMaxSeq];
-  __shared__ int s_scan[kPlanThreads / 32 + 1];
-  __shared__ unsigned long long s_tot;
+  __shared__ int64_t s_scan[2 * kPlanThreads / 32];
   pdl_wait();
   const int tid = threadIdx.x;
   const int sh = __ffs(a.page_size) - 1, pm = a.page_size - 1;
   const long long cap = (long long)a.max_blocks << sh;
-  if (tid == 0) s_tot = 0;
-  __syncthreads();
   const int n_free = *a.n_free;
   const int per = (a.n_seq + kPlanThreads - 1) / kPlanThreads;
   int n = 0, bits = (n_free < 0 || n_free > a.n_pages) ? HC_DEV_INDEX : 0;
@@ -155,15 +173,16 @@ __global__ void __launch_bounds__(kPlanThreads) release_pages_kernel(PagePlanArg
     else give[i] = ((len + pm) >> sh) - ((keep[i] + pm) >> sh);
     n += give[i];
   }
-  if (n) atomicAdd(&s_tot, (unsigned long long)n);
+  int64_t first0, total0, none0, none1;
+  scan_pair(n, 0, s_scan, first0, none0, total0, none1);
   const int bad = __syncthreads_or(bits);
-  bits = bad ? HC_DEV_INDEX : (s_tot > (unsigned long long)(a.n_pages - n_free) ? HC_DEV_CAPACITY : 0);
+  bits = bad ? HC_DEV_INDEX : (total0 > a.n_pages - n_free ? HC_DEV_CAPACITY : 0);
   if (bits) {  // nothing is given back
     if (tid == 0 && a.status) atomicOr(a.status, bits);
     return;
   }
-  const int total = (int)s_tot;
-  int dummy, first = block_exclusive_scan(n, s_scan, dummy);
+  const int total = (int)total0;
+  int first = (int)first0;
 #pragma unroll
   for (int i = 0; i < kPlanPer; ++i) {
     const int b = tid * per + i;

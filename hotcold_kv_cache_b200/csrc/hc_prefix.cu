@@ -79,36 +79,42 @@ __global__ void __launch_bounds__(kSimtThreads, 2) prefix_simt_kernel(PrefixArgs
       const int k0 = kt * kSimtK;
       bool odd = false;  // a value that is not finite
       __syncthreads();
-      for (int x = tid; x < kSimtK * CPR; x += kSimtThreads) {
-        const int r = x / CPR, c = x % CPR, key = k0 + r;
-        float fk[VEC], fv[VEC];
+      // a thread takes one 16-byte column of every 8th (16th) row; four rows' loads in flight at a time
+      constexpr int RS = kSimtThreads / CPR, LB = 4;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) fk[e] = fv[e] = 0.f;
-        const T *kr = nullptr, *vr = nullptr;
-        if (key < p.kend) {
-          if (p.own) {
-            const int page = a.block_table[(size_t)p.b * a.max_blocks + (key >> sh)];
-            if (page >= 0 && page < a.n_pages) {
-              const size_t off = (((size_t)page * ls.Hk + p.h) * a.page_size + (key & (a.page_size - 1))) * D;
-              kr = reinterpret_cast<const T*>(a.k_pages) + off;
-              vr = reinterpret_cast<const T*>(a.v_pages) + off;
-            } else if (a.status) {
-              atomicOr(a.status, HC_DEV_INDEX);
+      for (int r0 = 0; r0 < kSimtK; r0 += RS * LB) {
+        uint4 uk[LB], uv[LB];
+#pragma unroll
+        for (int u = 0; u < LB; ++u) {
+          const int key = k0 + r0 + u * RS + tid / CPR, c = tid % CPR;
+          const T *kr = nullptr, *vr = nullptr;
+          if (key < p.kend) {
+            if (p.own) {
+              const int page = a.block_table[(size_t)p.b * a.max_blocks + (key >> sh)];
+              if (page >= 0 && page < a.n_pages) {
+                const size_t off = (((size_t)page * ls.Hk + p.h) * a.page_size + (key & (a.page_size - 1))) * D;
+                kr = reinterpret_cast<const T*>(a.k_pages) + off;
+                vr = reinterpret_cast<const T*>(a.v_pages) + off;
+              } else if (a.status) {
+                atomicOr(a.status, HC_DEV_INDEX);
+              }
+            } else if (!a.mask || a.mask[key]) {
+              kr = reinterpret_cast<const T*>(a.pk) + p.h * a.pk_sh + (int64_t)key * a.pk_st;
+              vr = reinterpret_cast<const T*>(a.pv) + p.h * a.pv_sh + (int64_t)key * a.pv_st;
             }
-          } else if (!a.mask || a.mask[key]) {
-            kr = reinterpret_cast<const T*>(a.pk) + p.h * a.pk_sh + (int64_t)key * a.pk_st;
-            vr = reinterpret_cast<const T*>(a.pv) + p.h * a.pv_sh + (int64_t)key * a.pv_st;
           }
-        }
-        if (kr) {
-          unpack16<DT>(reinterpret_cast<const uint4*>(kr)[c], fk);
-          unpack16<DT>(reinterpret_cast<const uint4*>(vr)[c], fv);
+          uk[u] = kr ? reinterpret_cast<const uint4*>(kr)[c] : make_uint4(0u, 0u, 0u, 0u);
+          uv[u] = vr ? reinterpret_cast<const uint4*>(vr)[c] : make_uint4(0u, 0u, 0u, 0u);
         }
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          sK[r * KS + c * VEC + e] = fk[e];
-          sV[r * D + c * VEC + e] = fv[e];
-          odd |= !isfinite(fv[e]);
+        for (int u = 0; u < LB; ++u) {
+          const int r = r0 + u * RS + tid / CPR, c = tid % CPR;
+          *reinterpret_cast<uint4*>(sK + r * KS + c * VEC) = uk[u];
+          *reinterpret_cast<uint4*>(sV + r * D + c * VEC) = uv[u];
+          float f[VEC];
+          unpack16<DT>(uv[u], f);
+#pragma unroll
+          for (int e = 0; e < VEC; ++e) odd |= !isfinite(f[e]);
         }
       }
       // a causal tile whose hidden keys hold values that are not finite takes the careful product
@@ -233,11 +239,10 @@ __global__ void __launch_bounds__(kSimtThreads, 2) prefix_simt_kernel(PrefixArgs
 // A row with no attended key at all is 0 with a log-sum of -inf. Bound by the partial results it reads
 // (from L2) and, for a decode step, by its launch and three dependent reads.
 // ----------------------------------------------------------------------------------------
-constexpr int kMergeThreads = 256;
 constexpr int kMaxCtas = 448;     // CTAs a call's work is divided among
 constexpr int kMergeList = 512;   // >= partial results of a row: one per CTA and one more per group of the row (17)
 
-template <int DT, int D>
+template <int DT, int D, int kMergeThreads>
 __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(PrefixArgs a, LineShape s, const int64_t* hdr,
                                                                      const float2* ml, const float* part) {
   using E = Elem<DT>;
@@ -433,8 +438,12 @@ static cudaError_t prefix_t(const PrefixArgs& a, void* scratch, cudaStream_t str
     e = launch_prefix_mma(a, s, DT, D, hdr, ml, part, stream);
   }
   if (e != cudaSuccess) return e;
-  return launch_pdl(prefix_merge_kernel<DT, D>, dim3((unsigned)a.T, (unsigned)a.Hk), dim3(kMergeThreads), 0, stream, a, s,
-                    (const int64_t*)hdr, (const float2*)ml, (const float*)part);
+  // few rows have many blocks each: wide CTAs take shares of them (8 rows of 68 blocks: 21 us with 256 threads);
+  // many rows have few, and fill the GPU by themselves
+  const bool wide = (int64_t)a.T * a.Hk < 2048;
+  return launch_pdl(wide ? prefix_merge_kernel<DT, D, 512> : prefix_merge_kernel<DT, D, 128>,
+                    dim3((unsigned)a.T, (unsigned)a.Hk), dim3(wide ? 512 : 128), 0, stream, a, s, (const int64_t*)hdr,
+                    (const float2*)ml, (const float*)part);
 }
 
 cudaError_t launch_prefix_attention(const PrefixArgs& a, int dtype, int D, void* scratch, cudaStream_t stream) {

@@ -69,7 +69,7 @@ __device__ __forceinline__ LineCost line_cost(const LineShape& s, int rows) {
 }
 
 // The shortest stretch is >= every a: no CTA between a group's first and last is without a tile.
-__device__ __forceinline__ int min_stretch(const LineShape& s) { return s.dup == 1 ? 1 : 5; }
+__device__ __forceinline__ int min_stretch(const LineShape& s) { return s.dup == 1 ? 2 : 7; }
 
 struct Piece {
   bool own;         // suffix (own pages) or prefix

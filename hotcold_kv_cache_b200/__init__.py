@@ -28,6 +28,8 @@ __all__ = [
     "release_pages",
     "append_pages",
     "shared_prefix_attention",
+    "SharedPrefixCache",
+    "build_shared_prefix_cache",
 ]
 
 
@@ -39,6 +41,9 @@ def __getattr__(name):
         from . import prefix
         globals()[name] = getattr(prefix, name)  # found without this function from now on
         return globals()[name]
+    if name in ("SharedPrefixCache", "build_shared_prefix_cache"):
+        from . import prefix_cache
+        return getattr(prefix_cache, name)
     if name == "KVController":
         from .controller import KVController
         return KVController

@@ -7,7 +7,9 @@ runs. A further multi-token forward on a non-empty cache (a prompt sent in
 chunks, which the reference rejects) attends to the kept hot tokens and joins
 them (KVController.prefill_chunk). A one-token decode forward runs the sm_100a
 hot path of the layer: RoPE + append, the scheduled retrieval, compression,
-attention over [held | hot] — without host synchronisation.
+attention over [held | hot] — without host synchronisation. Layers of a
+SharedPrefixCache go to prefix_cache.shared_prefix_forward, with or without an
+active controller.
 """
 
 from __future__ import annotations
@@ -23,6 +25,7 @@ from transformers.models.llama import modeling_llama
 from .cache import HotColdLayer
 from .datatypes import _canon_br_2d, _canon_kv_4d
 from .kernels import triton_evict_attention_forward
+from .prefix_cache import SharedPrefixCache, shared_prefix_forward
 
 ACTIVE_KVCTRL = None
 ACTIVE_ROTARY_EMB = None  # set to model.model.rotary_emb
@@ -82,6 +85,8 @@ def install_monkeypatch(enable_debug: bool = True):
     def patched_forward(self, hidden_states: torch.Tensor, position_embeddings: Tuple[torch.Tensor, torch.Tensor],
                         attention_mask: Optional[torch.Tensor] = None, past_key_values: Optional[Cache] = None,
                         cache_position: Optional[torch.LongTensor] = None, **kwargs):
+        if isinstance(past_key_values, SharedPrefixCache):
+            return shared_prefix_forward(self, hidden_states, position_embeddings, attention_mask, past_key_values)
         kvctrl = ACTIVE_KVCTRL
         if kvctrl is None:
             return _ORIG(self, hidden_states=hidden_states, position_embeddings=position_embeddings,

@@ -1,0 +1,238 @@
+"""A transformers cache for a batch of sequences behind one shared prefix.
+
+    cache = build_shared_prefix_cache(model)
+    model(document_ids, past_key_values=cache)          # (1, P): the prefix, run once
+    cache.begin(n_seq=16, max_new_tokens=512)            # sixteen requests behind it
+    model(question_ids, past_key_values=cache)          # (16, T); cache.next_lens([...]) first where they are ragged
+    model(next_ids, past_key_values=cache)              # (16, 1), and so on
+
+It needs install_monkeypatch(): the patched LlamaAttention.forward hands layers of this cache to
+`shared_prefix_forward`. The prefix's keys and values exist once; the sequences' own tokens are in pages
+(plan_pages, append_pages) and every step reads the prefix once for the whole batch
+(shared_prefix_attention). Nothing is compressed or evicted: it is the exact counterpart of
+build_hotcold_cache for many short requests on one long document. The reference has no counterpart.
+"""
+
+from __future__ import annotations
+
+from typing import List, Optional, Sequence, Tuple
+
+import torch
+import torch.nn.functional as F
+from transformers.cache_utils import Cache, CacheLayerMixin
+
+from .prefix import PagePlan, append_pages, plan_pages, release_pages, shared_prefix_attention
+
+
+class SharedPrefixLayer(CacheLayerMixin):
+    """One layer: the prefix's post-RoPE keys and values (Hk, P, D) and the pages of the sequences' own."""
+    is_compileable = False
+
+    def __init__(self, owner: "SharedPrefixCache", layer_idx: int):
+        super().__init__()
+        self.owner, self.layer_idx = owner, layer_idx
+        self.prefix_k: Optional[torch.Tensor] = None
+        self.prefix_v: Optional[torch.Tensor] = None
+        self.k_pages: Optional[torch.Tensor] = None
+        self.v_pages: Optional[torch.Tensor] = None
+        self.is_initialized = False
+
+    @property
+    def keys(self):
+        return self.prefix_k
+
+    @keys.setter
+    def keys(self, _):
+        pass
+
+    @property
+    def values(self):
+        return self.prefix_v
+
+    @values.setter
+    def values(self, _):
+        pass
+
+    def lazy_initialization(self, key_states, value_states=None):
+        self.is_initialized = True
+
+    def update(self, *args, **kwargs):
+        raise RuntimeError("a shared-prefix cache is read by the patched attention: call install_monkeypatch() first")
+
+    def get_mask_sizes(self, cache_position) -> Tuple[int, int]:
+        q = cache_position if isinstance(cache_position, int) else int(cache_position.shape[0])
+        return int(self.get_seq_length() + q), 0
+
+    def get_seq_length(self) -> int:
+        """Prefix tokens plus the longest sequence's own."""
+        return self.owner.prefix_len + max(self.owner.host_lens, default=0)
+
+    def get_max_cache_shape(self) -> int:
+        return -1
+
+
+class SharedPrefixCache(Cache):
+    def __init__(self, n_layers: int, inv_freq: torch.Tensor, rope_scaling: float = 1.0, page_size: int = 64):
+        if page_size < 16 or page_size > 256 or page_size & (page_size - 1):
+            raise ValueError(f"page_size must be a power of two from 16 to 256, not {page_size}")
+        super().__init__(layers=[SharedPrefixLayer(self, i) for i in range(n_layers)])
+        self.inv_freq, self.rope_scaling, self.page_size = inv_freq, float(rope_scaling), int(page_size)
+        self.prefix_len = 0
+        self.prefix_mask: Optional[torch.Tensor] = None
+        self.n_seq = 0  # 0 until begin()
+        self.host_lens: List[int] = []  # own tokens of each sequence, as the device's lens
+        self.plan: Optional[PagePlan] = None
+        self._next: Optional[List[int]] = None
+        self._rows: Optional[torch.Tensor] = None
+
+    # ------------------------------------------------------------------ setup
+    def set_prefix(self, layer_idx: int, k: torch.Tensor, v: torch.Tensor):
+        """Post-RoPE keys and values (Hk, P, D) of the prefix in one layer; read in place, not copied, where
+        their rows are 16-byte aligned."""
+        layer = self.layers[layer_idx]
+        if layer.prefix_k is not None:
+            raise RuntimeError("the prefix is set: it goes through the model in one forward, before begin()")
+        if k.shape != v.shape or k.dim() != 3:
+            raise ValueError("prefix keys and values must share a shape (Hk, P, D)")
+
+        def rows(x):
+            per = 16 // x.element_size()
+            ok = x.stride(2) == 1 and x.stride(0) % per == 0 and x.stride(1) % per == 0 and x.data_ptr() % 16 == 0
+            return x if ok and x.stride(0) > 0 and x.stride(1) > 0 else x.contiguous()
+
+        layer.prefix_k, layer.prefix_v = rows(k), rows(v)
+        layer.is_initialized = True
+        self.prefix_len = int(k.shape[1])
+
+    def begin(self, n_seq: int, max_new_tokens: int, pool_tokens: Optional[int] = None,
+              prefix_mask: Optional[torch.Tensor] = None):
+        """n_seq empty sequences behind the prefix, each with at most max_new_tokens own tokens; the pages of
+        all hold pool_tokens (default: enough for every sequence's most). prefix_mask (P) bool leaves prefix
+        tokens out."""
+        first = self.layers[0]
+        if first.prefix_k is None:
+            raise RuntimeError("begin() comes after the prefix's forward")
+        if n_seq < 1 or max_new_tokens < 1:
+            raise ValueError("begin() needs at least one sequence and one new token")
+        dev, (Hk, _, D) = first.prefix_k.device, first.prefix_k.shape
+        ps = self.page_size
+        self.n_seq, self.max_blocks = int(n_seq), -(-int(max_new_tokens) // ps)
+        most = self.n_seq * self.max_blocks
+        self.n_pages = most if pool_tokens is None else max(1, min(most, -(-int(pool_tokens) // ps)))
+        z = dict(dtype=torch.int32, device=dev)
+        self.lens = torch.zeros(self.n_seq, **z)
+        self.block_table = torch.full((self.n_seq, self.max_blocks), -1, **z)
+        self.free_pages = torch.arange(self.n_pages, **z)
+        self.n_free = torch.full((1,), self.n_pages, **z)
+        self.status = torch.zeros(1, **z)
+        self.prefix_mask = None if prefix_mask is None else prefix_mask.to(device=dev, dtype=torch.uint8).contiguous()
+        self.inv_freq = self.inv_freq.detach().to(device=dev, dtype=torch.float32).contiguous()
+        for layer in self.layers:
+            if layer.prefix_k is None:
+                raise RuntimeError("begin() comes after the prefix's forward")
+            layer.k_pages = torch.empty((self.n_pages, Hk, ps, D), dtype=layer.prefix_k.dtype, device=dev)
+            layer.v_pages = torch.empty_like(layer.k_pages)
+        self.host_lens = [0] * self.n_seq
+        self._next = self.plan = None
+
+    # ------------------------------------------------------------------ steps
+    def next_lens(self, lens: Sequence[int]):
+        """How many of the next forward's tokens of each row are real (the row's first ones; the rest is
+        padding, whose outputs mean nothing). Without it all are."""
+        lens = [int(x) for x in lens]
+        if len(lens) != self.n_seq or min(lens) < 0:
+            raise ValueError(f"next_lens needs {self.n_seq} lengths, none negative")
+        self._next = lens
+
+    def _pages(self, lens) -> int:
+        return sum(-(-x // self.page_size) for x in lens)
+
+    def start_step(self, batch: int, tokens: int):
+        """Page plan of a forward of (batch, tokens), shared by its layers."""
+        if batch != self.n_seq:
+            raise ValueError(f"the batch has {batch} rows, the cache {self.n_seq} sequences")
+        new = self._next if self._next is not None else [tokens] * self.n_seq
+        if max(new) > tokens:
+            raise ValueError(f"next_lens names {max(new)} tokens of a row of {tokens}")
+        after = [a + b for a, b in zip(self.host_lens, new)]
+        if max(after) > self.max_blocks * self.page_size or self._pages(after) > self.n_pages:
+            raise RuntimeError(f"the pages do not hold this step: {self._pages(after)} of {self.n_pages} pages, longest "
+                               f"sequence {max(after)} of {self.max_blocks * self.page_size} tokens")
+        dev = self.lens.device
+        n = batch * tokens
+        uniform = min(new) == tokens
+        add = torch.full((self.n_seq,), tokens, dtype=torch.int32, device=dev) if uniform else \
+            torch.tensor(new, dtype=torch.int32, device=dev)
+        p = self.plan = plan_pages(self.lens, add, self.block_table, self.free_pages, self.n_free, self.page_size, n,
+                                   base_pos=self.prefix_len)
+        # packed row t comes from row seq * tokens + its place in the sequence; row n stands for none
+        self._rows = None
+        if not uniform:
+            seq = p.seq_ids.long()
+            place = torch.arange(n, device=dev) - p.cu_new[seq.clamp(min=0)]
+            self._rows = torch.where(seq >= 0, seq * tokens + place, n)
+        self.host_lens, self._next = after, None
+
+    def attend(self, layer_idx: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scaling: float) -> torch.Tensor:
+        """The layer's step after start_step: q (B*T,Hq,D), k and v (B*T,Hk,D) pre-RoPE; returns (B*T,Hq,D)."""
+        layer, p, rows = self.layers[layer_idx], self.plan, self._rows
+        n = q.shape[0]
+        if rows is not None:
+            at = rows.clamp(max=n - 1)
+            q, k, v = q.index_select(0, at), k.index_select(0, at), v.index_select(0, at)
+        q = append_pages(q, k, v, p.slots, p.positions, layer.k_pages, layer.v_pages, inv_freq=self.inv_freq,
+                         rope_scaling=self.rope_scaling, status=self.status)
+        out = shared_prefix_attention(q, layer.prefix_k, layer.prefix_v, layer.k_pages, layer.v_pages, self.block_table,
+                                      p.lens, p.cu_new, scaling, prefix_mask=self.prefix_mask, status=self.status)
+        if rows is None:
+            return out
+        back = torch.zeros((n + 1,) + out.shape[1:], dtype=out.dtype, device=out.device)
+        back.index_copy_(0, rows, out)  # the padding rows all land in the last one
+        return back[:n]
+
+    def release(self, keep_lens: Sequence[int]):
+        """Sequence b keeps its first keep_lens[b] own tokens (0 frees it for another request)."""
+        keep = [int(x) for x in keep_lens]
+        if len(keep) != self.n_seq or any(x < 0 or x > n for x, n in zip(keep, self.host_lens)):
+            raise ValueError(f"release keeps {keep} of {self.host_lens} tokens")
+        release_pages(self.lens, torch.tensor(keep, dtype=torch.int32, device=self.lens.device), self.block_table,
+                      self.free_pages, self.n_free, self.page_size, status=self.status)
+        self.host_lens = keep
+
+    def device_status(self) -> int:
+        """OR of the HC_DEV_* bits of the steps so far (synchronises)."""
+        return int(self.status) | (int(self.plan.status) if self.plan is not None else 0)
+
+
+def build_shared_prefix_cache(model, page_size: int = 64) -> SharedPrefixCache:
+    """A SharedPrefixCache for a Llama model: its layer count and rotary parameters."""
+    rot = model.model.rotary_emb
+    return SharedPrefixCache(int(model.config.num_hidden_layers), rot.inv_freq, float(getattr(rot, "attention_scaling", 1.0)),
+                             page_size)
+
+
+def shared_prefix_forward(attn, hidden_states, position_embeddings, attention_mask, cache: SharedPrefixCache):
+    """LlamaAttention.forward over a SharedPrefixCache: before begin() the prefix's forward (transformers' RoPE and
+    stock causal attention, as the patched prompt forward), after it the batch's step."""
+    from transformers.models.llama import modeling_llama
+    b, t, _ = hidden_states.shape
+    li, d = int(attn.layer_idx), int(attn.head_dim)
+    q = attn.q_proj(hidden_states).view(b, t, -1, d)
+    k = attn.k_proj(hidden_states).view(b, t, -1, d)
+    v = attn.v_proj(hidden_states).view(b, t, -1, d)
+    if cache.n_seq == 0:
+        if b != 1:
+            raise ValueError("the prefix goes through the model as one sequence; begin() then opens the batch")
+        qt, kt, vt = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
+        cos, sin = position_embeddings
+        qt, kt = modeling_llama.apply_rotary_pos_emb(qt, kt, cos, sin)
+        cache.set_prefix(li, kt[0], vt[0])
+        rep = qt.shape[1] // kt.shape[1]
+        kr, vr = (modeling_llama.repeat_kv(kt, rep), modeling_llama.repeat_kv(vt, rep)) if rep > 1 else (kt, vt)
+        out = F.scaled_dot_product_attention(qt, kr, vr, attn_mask=attention_mask, dropout_p=0.0,
+                                             is_causal=attention_mask is None and t > 1)
+        return attn.o_proj(out.transpose(1, 2).reshape(b, t, -1)), None
+    if li == 0:
+        cache.start_step(b, t)
+    out = cache.attend(li, q.reshape(b * t, -1, d), k.reshape(b * t, -1, d), v.reshape(b * t, -1, d), float(attn.scaling))
+    return attn.o_proj(out.reshape(b, t, -1)), None

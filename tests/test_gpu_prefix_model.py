@@ -1,0 +1,155 @@
+"""The shared-prefix cache through the patched Llama forward: every request's logits equal those of the stock model on
+[prefix + its own tokens] alone."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+CFG = dict(vocab_size=500, hidden_size=512, intermediate_size=1024, num_hidden_layers=3, num_attention_heads=8,
+           num_key_value_heads=2, head_dim=64, rope_theta=500000.0, max_position_embeddings=4096)
+
+
+def setup(dtype):
+    from transformers import LlamaConfig, LlamaForCausalLM
+    torch.manual_seed(3)
+    model = LlamaForCausalLM(LlamaConfig(**CFG)).eval().to(device="cuda", dtype=dtype)
+    g = torch.Generator().manual_seed(4)
+    ids = lambda *s: torch.randint(0, CFG["vocab_size"], s, generator=g).cuda()  # noqa: E731
+    return model, ids
+
+
+def stock(model, prefix, own):
+    """Logits of the own tokens in one stock forward over [prefix | own]."""
+    out = model(input_ids=torch.cat([prefix, own], 1), use_cache=False)
+    return out.logits[0, prefix.shape[1]:].float()
+
+
+# a 3-layer model in fp32: sums of up to 1024 terms in other orders, 1e-4 of logits of order 1; in 16 bits each of the 3
+# layers rounds its activations (2^-8 in bf16) in two places on other paths: 16 roundings, 2^-4, and 2^-7 for fp16
+TOL = {torch.float32: 1e-4, torch.float16: 2.0 ** -7, torch.bfloat16: 2.0 ** -4}
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+def test_requests_behind_a_document(dtype):
+    import hotcold_kv_cache_b200 as hc
+    model, ids = setup(dtype)
+    prefix, B = ids(1, 700), 3
+    q = ids(B, 40)
+    lens = [40, 7, 23]
+    steps = [ids(B, 1) for _ in range(4)]
+    hc.install_monkeypatch(enable_debug=False)
+    try:
+        with torch.inference_mode():
+            cache = hc.build_shared_prefix_cache(model, page_size=16)
+            first = model(input_ids=prefix, past_key_values=cache, use_cache=True).logits[0].float()
+            cache.begin(B, max_new_tokens=64)
+            cache.next_lens(lens)
+            got = [[x] for x in model(input_ids=q, past_key_values=cache, use_cache=True).logits.float()]
+            got = [[x[0][:n]] for x, n in zip(got, lens)]
+            for s in steps:
+                o = model(input_ids=s, past_key_values=cache, use_cache=True).logits.float()
+                for b in range(B):
+                    got[b].append(o[b])
+            assert cache.device_status() == 0 and cache.host_lens == [44, 11, 27]
+            assert cache.lens.tolist() == cache.host_lens and cache.get_seq_length() == 744
+            # request 1 ends; another question takes its place
+            cache.release([44, 0, 27])
+            q2 = ids(1, 9)
+            pad = torch.zeros(B, 9, dtype=torch.long, device="cuda")
+            pad[1] = q2
+            cache.next_lens([0, 9, 0])
+            late = model(input_ids=pad, past_key_values=cache, use_cache=True).logits[1].float()
+            assert cache.device_status() == 0
+    finally:
+        hc.uninstall_monkeypatch()
+    with torch.inference_mode():
+        tol = TOL[dtype]
+        ref = model(input_ids=prefix, use_cache=False).logits[0].float()
+        assert (first - ref).abs().max() <= tol * ref.abs().max()
+        for b in range(B):
+            own = torch.cat([q[b:b + 1, :lens[b]]] + [s[b:b + 1] for s in steps], 1)
+            ref = stock(model, prefix, own)
+            assert (torch.cat(got[b]) - ref).abs().max() <= tol * ref.abs().max()
+        ref = stock(model, prefix, q2)
+        assert (late - ref).abs().max() <= tol * ref.abs().max()
+
+
+def test_decode_step_as_a_graph():
+    """A uniform decode step captured once and replayed: the tables advance on the device."""
+    import hotcold_kv_cache_b200 as hc
+    model, ids = setup(torch.float16)
+    prefix, B = ids(1, 300), 4
+    q = ids(B, 5)
+    steps = [ids(B, 1) for _ in range(4)]
+
+    def run(graph):
+        out = []
+        cache = hc.build_shared_prefix_cache(model, page_size=16)
+        model(input_ids=prefix, past_key_values=cache, use_cache=True)
+        cache.begin(B, max_new_tokens=64)
+        model(input_ids=q, past_key_values=cache, use_cache=True)
+        if not graph:
+            for s in steps:
+                out.append(model(input_ids=s, past_key_values=cache, use_cache=True).logits.clone())
+        else:
+            tok = steps[0].clone()
+            side = torch.cuda.Stream()
+            side.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(side):  # warm up, then take the step back
+                model(input_ids=tok, past_key_values=cache, use_cache=True)
+                cache.release([5] * B)
+            torch.cuda.current_stream().wait_stream(side)
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g):
+                logits = model(input_ids=tok, past_key_values=cache, use_cache=True).logits
+            for s in steps:
+                tok.copy_(s)
+                g.replay()
+                out.append(logits.clone())
+            assert cache.lens.tolist() == [9] * B
+        assert cache.device_status() == 0
+        return torch.stack(out).float()
+
+    hc.install_monkeypatch(enable_debug=False)
+    try:
+        with torch.inference_mode():
+            assert torch.equal(run(True), run(False))
+    finally:
+        hc.uninstall_monkeypatch()
+
+
+def test_refusals():
+    import hotcold_kv_cache_b200 as hc
+    model, ids = setup(torch.float16)
+    hc.install_monkeypatch(enable_debug=False)
+    try:
+        with torch.inference_mode():
+            cache = hc.build_shared_prefix_cache(model, page_size=16)
+            with pytest.raises(RuntimeError):
+                cache.begin(2, 10)
+            with pytest.raises(ValueError):
+                model(input_ids=ids(2, 10), past_key_values=cache, use_cache=True)
+            model(input_ids=ids(1, 10), past_key_values=cache, use_cache=True)
+            with pytest.raises(RuntimeError):
+                model(input_ids=ids(1, 10), past_key_values=cache, use_cache=True)
+            with pytest.raises(ValueError):
+                cache.begin(0, 10)
+            cache.begin(2, 16)
+            with pytest.raises(ValueError):
+                model(input_ids=ids(3, 1), past_key_values=cache, use_cache=True)
+            with pytest.raises(ValueError):
+                cache.next_lens([1])
+            cache.next_lens([3, 1])
+            with pytest.raises(ValueError):
+                model(input_ids=ids(2, 2), past_key_values=cache, use_cache=True)
+            cache.next_lens([16, 1])
+            model(input_ids=ids(2, 16), past_key_values=cache, use_cache=True)
+            with pytest.raises(RuntimeError):
+                model(input_ids=ids(2, 1), past_key_values=cache, use_cache=True)  # the first sequence is full
+            with pytest.raises(ValueError):
+                cache.release([17, 1])
+    finally:
+        hc.uninstall_monkeypatch()
+    with pytest.raises(ValueError):
+        hc.build_shared_prefix_cache(model, page_size=24)

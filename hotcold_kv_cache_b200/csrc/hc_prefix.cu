@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(PrefixArgs 
       const int tiles = ceil_div(seq_keys(q, tok1), s.kt);
       rows = (tok1 - r * g.tt) * s.G, q0 = (t - q.cu - r * g.tt) * s.G;
       if (tiles > 0) {
-        const LineCost k = line_cost(s, min(q.n * s.G, s.rt));
+        const LineCost k = line_cost(s, min(q.n * s.G, s.rt), true);
         const int64_t v0 = hdr[1 + s_b] + ((int64_t)h * nr + r) * g.seq_group(s, q) + k.b;
         lo = line_div(v0, W), hi = line_div(v0 + (int64_t)(tiles - 1) * k.a, W);
         row = s.dup * ((int64_t)s.Hk * s.T * (s.P > 0 ? s.nch : 0) + (int64_t)q.cu * s.Hk + (int64_t)h * q.n + r * g.tt) * s.G;

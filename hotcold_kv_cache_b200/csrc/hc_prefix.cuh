@@ -62,10 +62,13 @@ cudaError_t launch_prefix_mma(const PrefixArgs& a, const LineShape& s, int dtype
 __host__ __device__ inline bool prefix_two_streams(int rows) { return rows > 64 && rows <= 128; }
 
 // fp32: alike. 16 bits, in units of about 0.55 us as measured on whole lines of one kind: tall row tiles
-// 2.7 us a key tile and 5.5 us to load Q and write the result, up to 64 rows 1.15 and 1.6 us.
-__device__ __forceinline__ LineCost line_cost(const LineShape& s, int rows) {
+// 2.8 us a key tile and 4.5 us to load Q and write the result (9.5 us behind causal tiles, where the streams
+// meet and V is looked through), up to 64 rows 1.15 and 1.6 us.
+__device__ __forceinline__ LineCost line_cost(const LineShape& s, int rows, bool own) {
   if (s.dup == 1) return {1, 1};
-  return rows > 128 ? LineCost{5, 10} : prefix_two_streams(rows) ? LineCost{3, 8} : LineCost{2, 3};
+  if (rows > 128) return {5, own ? 17 : 8};
+  if (prefix_two_streams(rows)) return {3, own ? 12 : 6};
+  return {2, 3};
 }
 
 // The shortest stretch is >= every a: no CTA between a group's first and last is without a tile.
@@ -120,13 +123,13 @@ struct LineGeom {
     nrt = ceil_div(R, tt);
     ktp = ceil_div(s.P, s.kt);
     ct = ktp > 0 ? ceil_div(ktp, s.nch) : 0;
-    pre = line_cost(s, min(R * s.G, s.rt));
+    pre = line_cost(s, min(R * s.G, s.rt), false);
     head = ktp > 0 ? (int64_t)nrt * (ktp * pre.a + s.nch * pre.b) : 0;
     vpre = head * s.Hk;
   }
   __device__ int64_t seq_group(const LineShape& s, const SeqLens& q) const {  // one group of a sequence
     if (q.n <= 0 || q.len <= 0) return 0;
-    const LineCost c = line_cost(s, min(q.n * s.G, s.rt));
+    const LineCost c = line_cost(s, min(q.n * s.G, s.rt), true);
     return (int64_t)ceil_div(q.len, s.kt) * c.a + c.b;
   }
   __device__ int64_t seq_total(const LineShape& s, const SeqLens& q) const {
@@ -215,7 +218,7 @@ struct LineWalk {
   __device__ __forceinline__ void seq(const PrefixArgs& a, const LineShape& s, const LineGeom& g) {
     q = seq_lens(a, b);
     len = (int)g.seq_group(s, q);
-    cost = line_cost(s, min(q.n * s.G, s.rt));
+    cost = line_cost(s, min(q.n * s.G, s.rt), true);
     nr = len > 0 ? ceil_div(q.n, g.tt) : 0;
   }
   __device__ __forceinline__ LineWalk(const PrefixArgs& a, const LineShape& s, const LineGeom& g, const Stretch& st, int cta) {

@@ -36,6 +36,12 @@ class PagePlan(NamedTuple):
 _FN: dict = {}
 _SCRATCH_BYTES: dict = {}
 _I32, _I64 = torch.int32, torch.int64
+_CODE = {torch.float32: _lib.HC_F32, torch.float16: _lib.HC_F16, torch.bfloat16: _lib.HC_BF16}
+
+
+def _dtype_code(dtype) -> int:
+    code = _CODE.get(dtype)
+    return _lib.dtype_code(dtype) if code is None else code  # raises
 
 
 def _call(name: str, device, *args):
@@ -65,6 +71,13 @@ def _check(name: str, t: torch.Tensor, dtype, shape, device):
     raise ValueError(f"{name} must be contiguous")
 
 
+def _vector(name: str, t: torch.Tensor, dtype, n: int, dev):
+    """A contiguous CUDA tensor of n values of this dtype on device `dev` (a torch.device)."""
+    if t.dtype is dtype and t.numel() == n and t.get_device() == dev.index and t.is_contiguous():
+        return
+    _check(name, t, dtype, (n,), dev)
+
+
 def _cuda(name: str, t: torch.Tensor):
     if not t.is_cuda:
         raise ValueError(f"{name} must be a CUDA tensor: there is no CPU path")
@@ -89,11 +102,12 @@ def plan_pages(lens, new_lens, block_table, free_pages, n_free, page_size: int, 
     n_seq, max_blocks = block_table.shape
     i32, i64 = _I32, _I64
     n_tokens = int(n_tokens)
-    _check("lens", lens, i32, (n_seq,), dev)
-    _check("new_lens", new_lens, i32, (n_seq,), dev)
-    _check("block_table", block_table, i32, (n_seq, max_blocks), dev)
-    _check("free_pages", free_pages, i32, (free_pages.numel(),), dev)
-    _check("n_free", n_free, i32, (1,), dev)
+    n_pages = free_pages.numel()
+    _vector("lens", lens, i32, n_seq, dev)
+    _vector("new_lens", new_lens, i32, n_seq, dev)
+    _vector("block_table", block_table, i32, n_seq * max_blocks, dev)
+    _vector("free_pages", free_pages, i32, n_pages, dev)
+    _vector("n_free", n_free, i32, 1, dev)
     if n_tokens < 0:
         raise ValueError(f"n_tokens must not be negative, not {n_tokens}")
     if out is None:
@@ -101,15 +115,15 @@ def plan_pages(lens, new_lens, block_table, free_pages, n_free, page_size: int, 
                        torch.empty(n_tokens, dtype=i32, device=dev), torch.empty(n_tokens, dtype=i64, device=dev),
                        lens, n_free, torch.zeros(1, dtype=i32, device=dev))
     else:
-        _check("out.cu_new", out.cu_new, i32, (n_seq + 1,), dev)
-        _check("out.slots", out.slots, i64, (n_tokens,), dev)
-        _check("out.seq_ids", out.seq_ids, i32, (n_tokens,), dev)
-        _check("out.positions", out.positions, i64, (n_tokens,), dev)
-        _check("out.lens", out.lens, i32, (n_seq,), dev)
-        _check("out.n_free", out.n_free, i32, (1,), dev)
-        _check("out.status", out.status, i32, (1,), dev)
+        _vector("out.cu_new", out.cu_new, i32, n_seq + 1, dev)
+        _vector("out.slots", out.slots, i64, n_tokens, dev)
+        _vector("out.seq_ids", out.seq_ids, i32, n_tokens, dev)
+        _vector("out.positions", out.positions, i64, n_tokens, dev)
+        _vector("out.lens", out.lens, i32, n_seq, dev)
+        _vector("out.n_free", out.n_free, i32, 1, dev)
+        _vector("out.status", out.status, i32, 1, dev)
     _call("hc_plan_pages", dev, lens.data_ptr(), new_lens.data_ptr(), block_table.data_ptr(), free_pages.data_ptr(),
-          n_free.data_ptr(), n_seq, int(page_size), max_blocks, free_pages.numel(), n_tokens, int(base_pos),
+          n_free.data_ptr(), n_seq, int(page_size), max_blocks, n_pages, n_tokens, int(base_pos),
           out.lens.data_ptr(), out.n_free.data_ptr(), out.cu_new.data_ptr(), out.slots.data_ptr(),
           out.seq_ids.data_ptr(), out.positions.data_ptr(), out.status.data_ptr())
     return out
@@ -135,13 +149,15 @@ def release_pages(lens, keep_lens, block_table, free_pages, n_free, page_size: i
           _lib.ptr(status))
 
 
-def _rows16(t: torch.Tensor) -> torch.Tensor:
-    """`t` (rows, heads, D), or a contiguous copy, with 16-byte aligned rows of unit stride."""
+def _rows16(t: torch.Tensor):
+    """`t` (rows, heads, D), or a contiguous copy, with 16-byte aligned rows of unit stride; its address and
+    strides over rows and heads."""
     s0, s1, s2 = t.stride()
-    per = 16 // t.element_size()
-    if s2 == 1 and s0 % per == 0 and s1 % per == 0 and t.data_ptr() % 16 == 0:
-        return t
-    return t.clone(memory_format=torch.contiguous_format)
+    p = t.data_ptr()
+    if s2 != 1 or (p | (s0 | s1) * t.element_size()) & 15:
+        t = t.clone(memory_format=torch.contiguous_format)
+        (s0, s1, _), p = t.stride(), t.data_ptr()
+    return t, p, s0, s1
 
 
 def _pools(k_pages, v_pages, Hk: int, D: int, dtype, dev):
@@ -164,38 +180,37 @@ def append_pages(q, k, v, slots, positions, k_pages, v_pages, inv_freq=None, rop
     dev = _cuda("k", k)
     T, Hk, D = k.shape
     dtype = k.dtype
-    code = _lib.dtype_code(dtype)
+    code = _dtype_code(dtype)
     n_pages, page_size = _pools(k_pages, v_pages, Hk, D, dtype, dev)
     if v.shape != k.shape or v.dtype is not dtype or v.device != dev:
         raise ValueError("k and v must share shape, dtype and device")
-    _check("slots", slots, torch.int64, (T,), dev)
-    k, v = _rows16(k), _rows16(v)
-    Hq, qp, q_st, q_sh, qo = Hk, None, 0, 0, None
+    _vector("slots", slots, _I64, T, dev)
+    k, kp, k_st, k_sh = _rows16(k)
+    v, vp, v_st, v_sh = _rows16(v)
+    Hq, qp, q_st, q_sh, qo, pp, wp = Hk, None, 0, 0, None, None, None
     if inv_freq is not None:
-        _check("positions", positions, torch.int64, (T,), dev)
-        _check("inv_freq", inv_freq, torch.float32, (D // 2,), dev)
+        _vector("positions", positions, _I64, T, dev)
+        _vector("inv_freq", inv_freq, torch.float32, D // 2, dev)
+        pp, wp = positions.data_ptr(), inv_freq.data_ptr()
         if q is not None:
             if q.dim() != 3 or q.shape[0] != T or q.shape[2] != D or q.dtype is not dtype or q.device != dev:
                 raise ValueError(f"q must be ({T}, Hq, {D}) of k's dtype and device")
             Hq = q.shape[1]
-            q = _rows16(q)
+            q, qp, q_st, q_sh = _rows16(q)
             if q_out is None:
                 q_out = torch.empty((T, Hq, D), dtype=dtype, device=dev)
             else:
                 _check("q_out", q_out, dtype, (T, Hq, D), dev)
-            qp, qo = q.data_ptr(), q_out.data_ptr()
-            q_st, q_sh, _ = q.stride()
+            qo = q_out.data_ptr()
     elif q_out is not None:
         raise ValueError("q_out without inv_freq: the queries are not rotated")
     else:
         q_out = q
     if status is not None:
-        _check("status", status, torch.int32, (1,), dev)
-    k_st, k_sh, _ = k.stride()
-    v_st, v_sh, _ = v.stride()
-    _call("hc_append_pages", dev, qp, q_st, q_sh, k.data_ptr(), k_st, k_sh, v.data_ptr(), v_st, v_sh, qo,
-          slots.data_ptr(), None if inv_freq is None else positions.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(),
-          _lib.ptr(inv_freq), float(rope_scaling), T, Hq, Hk, D, page_size, n_pages, code, _lib.ptr(status))
+        _vector("status", status, _I32, 1, dev)
+    _call("hc_append_pages", dev, qp, q_st, q_sh, kp, k_st, k_sh, vp, v_st, v_sh, qo, slots.data_ptr(), pp,
+          k_pages.data_ptr(), v_pages.data_ptr(), wp, rope_scaling, T, Hq, Hk, D, page_size, n_pages, code,
+          _lib.ptr(status))
     return q_out
 
 
@@ -217,36 +232,39 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k_pages, v_pages, block_table
         raise ValueError(f"q must be (T, Hq, D), not {tuple(q.shape)}")
     T, Hq, D = q.shape
     dtype = q.dtype
-    code = _lib.dtype_code(dtype)
+    code = _dtype_code(dtype)
     Hk = k_pages.shape[1]
     n_pages, page_size = _pools(k_pages, v_pages, Hk, D, dtype, dev)
     n_seq, max_blocks = block_table.shape
     i32 = _I32
-    _check("block_table", block_table, i32, (n_seq, max_blocks), dev)
-    _check("lens", lens, i32, (n_seq,), dev)
-    _check("cu_new", cu_new, i32, (n_seq + 1,), dev)
-    P, pk, pv, st = 0, None, None, (0, 0, 0, 0)
+    _vector("block_table", block_table, i32, n_seq * max_blocks, dev)
+    _vector("lens", lens, i32, n_seq, dev)
+    _vector("cu_new", cu_new, i32, n_seq + 1, dev)
+    P, pk, pv, ks0, ks1, vs0, vs1 = 0, None, None, 0, 0, 0, 0
     if prefix_k is not None:
         P = prefix_k.shape[1]
-        for name, x in (("prefix_k", prefix_k), ("prefix_v", prefix_v)):
-            if x is None or x.shape != (Hk, P, D) or x.dtype is not dtype or x.device != dev:
-                raise ValueError(f"{name} must be ({Hk}, {P}, {D}) of q's dtype and device")
-            if x.stride(2) != 1:
-                raise ValueError(f"{name} must have unit stride over head_dim")
+        shape = (Hk, P, D)
+        if prefix_k.shape != shape or prefix_k.dtype is not dtype or prefix_k.device != dev:
+            raise ValueError(f"prefix_k must be {shape} of q's dtype and device")
+        if prefix_v is None or prefix_v.shape != shape or prefix_v.dtype is not dtype or prefix_v.device != dev:
+            raise ValueError(f"prefix_v must be {shape} of q's dtype and device")
         pk, pv = prefix_k.data_ptr(), prefix_v.data_ptr()
-        st = prefix_k.stride()[:2] + prefix_v.stride()[:2]
+        ks0, ks1, ks2 = prefix_k.stride()
+        vs0, vs1, vs2 = prefix_v.stride()
+        if ks2 != 1 or vs2 != 1:
+            raise ValueError("prefix_k and prefix_v must have unit stride over head_dim")
     if prefix_mask is not None:
         if prefix_mask.dtype is torch.bool:
             prefix_mask = prefix_mask.view(torch.uint8)
-        _check("prefix_mask", prefix_mask, torch.uint8, (P,), dev)
-    q = _rows16(q)
+        _vector("prefix_mask", prefix_mask, torch.uint8, P, dev)
+    q, qp, q_st, q_sh = _rows16(q)
     if out is None:
         out = torch.empty((T, Hq, D), dtype=dtype, device=dev)
     else:
         _check("out", out, dtype, (T, Hq, D), dev)
     lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if return_lse else None
     if status is not None:
-        _check("status", status, i32, (1,), dev)
+        _vector("status", status, i32, 1, dev)
     if T > 0:
         key = (dev.index, code, T, n_seq, Hq, Hk, D, P)
         nbytes = _SCRATCH_BYTES.get(key)
@@ -257,9 +275,8 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k_pages, v_pages, block_table
                 _SCRATCH_BYTES[key] = nbytes
         # this call's own: two streams, or two captured graphs, never share it
         scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
-        q_st, q_sh, _ = q.stride()
-        _call("hc_shared_prefix_attention", dev, q.data_ptr(), q_st, q_sh, pk, st[0], st[1], pv, st[2], st[3],
-              _lib.ptr(prefix_mask), k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), lens.data_ptr(),
-              cu_new.data_ptr(), out.data_ptr(), _lib.ptr(lse), _lib.ptr(status), T, n_seq, Hq, Hk, D, P, page_size,
-              max_blocks, n_pages, code, float(scaling), scratch.data_ptr(), scratch.numel())
+        _call("hc_shared_prefix_attention", dev, qp, q_st, q_sh, pk, ks0, ks1, pv, vs0, vs1, _lib.ptr(prefix_mask),
+              k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), lens.data_ptr(), cu_new.data_ptr(),
+              out.data_ptr(), _lib.ptr(lse), _lib.ptr(status), T, n_seq, Hq, Hk, D, P, page_size, max_blocks, n_pages,
+              code, scaling, scratch.data_ptr(), scratch.numel())
     return (out, lse) if return_lse else out

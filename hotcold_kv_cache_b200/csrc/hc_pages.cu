@@ -239,12 +239,12 @@ cudaError_t launch_release_pages(const PagePlanArgs& a, cudaStream_t stream) {
 // ----------------------------------------------------------------------------------------
 // Rotary append: x'[i] = x[i] cos - x[i + D/2] sin, x'[i + D/2] = x[i + D/2] cos + x[i] sin with the
 // angle position * inv_freq[i], for queries and keys; keys and values go to the row their slot names.
-// Bound by HBM: every element is read once and written once. A CTA takes one token; its 16-byte pairs
-// of chunks (i, i + D/2) are loaded while D/2 threads work out the token's angles.
-// The angle is reduced in 64 bits (a 32-bit product is off by 0.008 rad at position 131072) and the
-// rotation is done in 32 bits and rounded once.
+// Bound by HBM: every element is read once and written once. A CTA takes one token with a thread for each
+// pair of 16-byte chunks (i, i + D/2) of its rows, so that a token's loads are all in flight while D/2
+// threads work out its angles. The angle is reduced in 64 bits (a 32-bit product is off by 0.008 rad at
+// position 131072); the rotation is done in 32 bits and rounded once.
 // ----------------------------------------------------------------------------------------
-constexpr int kAppThreads = 256;
+constexpr int kAppThreads = 512;
 
 template <int DT, int D>
 __global__ void __launch_bounds__(kAppThreads) append_pages_kernel(PageAppendArgs a) {
@@ -255,69 +255,83 @@ __global__ void __launch_bounds__(kAppThreads) append_pages_kernel(PageAppendArg
   pdl_wait();
   const int t = blockIdx.x, tid = threadIdx.x;
   const int64_t slot = a.slots[t];
+  const int64_t pos = a.inv_freq && tid < H ? a.positions[t] : 0;
   if (slot < 0 || slot >= (int64_t)a.n_pages * a.page_size) {
     if (slot != -1 && tid == 0 && a.status) atomicOr(a.status, HC_DEV_INDEX);
     return;
   }
   const int64_t page = slot / a.page_size, row = slot % a.page_size;
-  if (a.inv_freq && tid < H) {
-    const double ang = (double)a.inv_freq[tid] * (double)a.positions[t];
-    const double n = rint(ang * 0.15915494309189535);  // 1 / (2 pi)
-    // 2 pi as the nearest double and what that leaves
-    const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, ang));
-    float c, s;
-    sincosf((float)r, &s, &c);
-    s_cos[tid] = c * a.rope_scaling;
-    s_sin[tid] = s * a.rope_scaling;
-  }
-  __syncthreads();
-  const T* q = reinterpret_cast<const T*>(a.q) + t * a.q_st;
-  const T* k = reinterpret_cast<const T*>(a.k) + t * a.k_st;
-  const T* v = reinterpret_cast<const T*>(a.v) + t * a.v_st;
-  T* qo = reinterpret_cast<T*>(a.q_out) + (size_t)t * a.Hq * D;
-  const int nq = a.q_out ? a.Hq : 0;
-  const int rot = (nq + a.Hk) * CH;
-  for (int x = tid; x < rot + a.Hk * CH; x += kAppThreads) {
+  const int nq = a.q_out ? a.Hq : 0, items = (nq + 2 * a.Hk) * CH;
+  bool first = true;
+  for (int x = tid; x - tid < items; x += blockDim.x) {
     const int hh = x / CH, c = x % CH;
-    const T* src;
-    T* dst;
+    const T* src = nullptr;
+    T* dst = nullptr;
     bool turn = a.inv_freq != nullptr;
-    if (hh < nq) {
-      src = q + hh * a.q_sh;
-      dst = qo + (size_t)hh * D;
-    } else if (hh < nq + a.Hk) {
-      const int h = hh - nq;
-      src = k + h * a.k_sh;
-      dst = reinterpret_cast<T*>(a.k_pages) + (((size_t)page * a.Hk + h) * a.page_size + row) * D;
-    } else {
-      const int h = hh - nq - a.Hk;
-      src = v + h * a.v_sh;
-      dst = reinterpret_cast<T*>(a.v_pages) + (((size_t)page * a.Hk + h) * a.page_size + row) * D;
-      turn = false;
-    }
-    uint4 lo = reinterpret_cast<const uint4*>(src)[c], hi = reinterpret_cast<const uint4*>(src + H)[c];
-    if (turn) {
-      float fl[VEC], fh[VEC];
-      unpack16<DT>(lo, fl);
-      unpack16<DT>(hi, fh);
-      alignas(16) T ol[VEC], oh[VEC];
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) {
-        const float cs = s_cos[c * VEC + e], sn = s_sin[c * VEC + e];
-        ol[e] = E::from_f(fl[e] * cs - fh[e] * sn);
-        oh[e] = E::from_f(fh[e] * cs + fl[e] * sn);
+    if (x < items) {
+      if (hh < nq) {
+        src = reinterpret_cast<const T*>(a.q) + t * a.q_st + hh * a.q_sh;
+        dst = reinterpret_cast<T*>(a.q_out) + ((size_t)t * a.Hq + hh) * D;
+      } else {
+        const int h = hh < nq + a.Hk ? hh - nq : hh - nq - a.Hk;
+        const size_t off = (((size_t)page * a.Hk + h) * a.page_size + row) * D;
+        if (hh < nq + a.Hk) {
+          src = reinterpret_cast<const T*>(a.k) + t * a.k_st + h * a.k_sh;
+          dst = reinterpret_cast<T*>(a.k_pages) + off;
+        } else {
+          src = reinterpret_cast<const T*>(a.v) + t * a.v_st + h * a.v_sh;
+          dst = reinterpret_cast<T*>(a.v_pages) + off;
+          turn = false;
+        }
       }
-      lo = *reinterpret_cast<uint4*>(ol);
-      hi = *reinterpret_cast<uint4*>(oh);
     }
-    reinterpret_cast<uint4*>(dst)[c] = lo;
-    reinterpret_cast<uint4*>(dst + H)[c] = hi;
+    uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+    if (src) {
+      lo = reinterpret_cast<const uint4*>(src)[c];
+      hi = reinterpret_cast<const uint4*>(src + H)[c];
+    }
+    if (first && a.inv_freq) {
+      if (tid < H) {
+        const double ang = (double)a.inv_freq[tid] * (double)pos;
+        const double n = rint(ang * 0.15915494309189535);  // 1 / (2 pi)
+        // 2 pi as the nearest double and what that leaves
+        const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, ang));
+        float cs, sn;
+        sincosf((float)r, &sn, &cs);
+        s_cos[tid] = cs * a.rope_scaling;
+        s_sin[tid] = sn * a.rope_scaling;
+      }
+      __syncthreads();
+    }
+    first = false;
+    if (src) {
+      if (turn) {
+        float fl[VEC], fh[VEC];
+        unpack16<DT>(lo, fl);
+        unpack16<DT>(hi, fh);
+        alignas(16) T ol[VEC], oh[VEC];
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+          const float cs = s_cos[c * VEC + e], sn = s_sin[c * VEC + e];
+          ol[e] = E::from_f(fl[e] * cs - fh[e] * sn);
+          oh[e] = E::from_f(fh[e] * cs + fl[e] * sn);
+        }
+        lo = *reinterpret_cast<uint4*>(ol);
+        hi = *reinterpret_cast<uint4*>(oh);
+      }
+      reinterpret_cast<uint4*>(dst)[c] = lo;
+      reinterpret_cast<uint4*>(dst + H)[c] = hi;
+    }
   }
 }
 
 template <int DT, int D>
 static cudaError_t append_pages_t(const PageAppendArgs& a, cudaStream_t stream) {
-  return launch_pdl(append_pages_kernel<DT, D>, dim3((unsigned)a.n_tokens), dim3(kAppThreads), 0, stream, a);
+  const int items = ((a.q_out ? a.Hq : 0) + 2 * a.Hk) * (D / 2) / (DT == HC_F32 ? 4 : 8);
+  int threads = (items + 31) / 32 * 32;
+  if (threads < D / 2) threads = D / 2;
+  if (threads > kAppThreads) threads = kAppThreads;
+  return launch_pdl(append_pages_kernel<DT, D>, dim3((unsigned)a.n_tokens), dim3((unsigned)threads), 0, stream, a);
 }
 
 cudaError_t launch_append_pages(const PageAppendArgs& a, int dtype, int D, cudaStream_t stream) {

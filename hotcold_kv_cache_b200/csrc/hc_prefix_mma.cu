@@ -201,6 +201,18 @@ struct PieceRing {
   const Piece* e;
   uint64_t *full, *empty;
   uint32_t k;
+  // Whether the next piece is listed, for the whole warp.
+  __device__ __forceinline__ bool listed() const {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(smem_u32(&full[k % kPieces])), "r"((k / kPieces) & 1)
+        : "memory");
+    return __all_sync(0xffffffffu, ok);
+  }
   // Copies the next piece; false after the last. `lanes`: the threads of the warp that read it.
   __device__ __forceinline__ bool next(Piece& p, uint32_t lanes, bool first) {
     mbar_wait_long(&full[k % kPieces], (k / kPieces) & 1);
@@ -799,18 +811,23 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
     uint32_t base = 0, next_base = 0, nt = 0, turn = 0, meets = 0;
     Piece p, q;
     Part tq;
-    // the next piece of this stream; `base` goes along
-    auto advance = [&]() -> bool {
-      for (;;) {
-        if (!ring.next(q, 0xffffffffu, lane == 0)) return false;
+    // The next piece of this stream; `base` goes along. A stream that still has work on its piece may not
+    // wait here: it can have many pieces to pass by, which are listed only as the others get on, and those may
+    // need this stream's work (its share of the ring, the meetings). So it looks ahead as far as pieces are
+    // listed, and waits only once it is done.
+    enum { kNone = 0, kHave, kEnd };  // not listed yet; found; no more
+    auto advance = [&](bool wait) -> int {
+      while (wait || ring.listed()) {
+        if (!ring.next(q, 0xffffffffu, lane == 0)) return kEnd;
         tq = piece_part(q, G, x, turn);
         base = next_base;
         next_base += 2 * tq.tiles;
         if (tq.rows <= 64) ++turn;
-        if (tq.mode != kSkip) return true;
+        if (tq.mode != kSkip) return kHave;
         // too few key tiles for this stream: its block of partial rows holds nothing
         if (prefix_two_streams(tq.rows) && r < tq.rows) ml[q.row0 + tq.rows + r] = make_float2(kNegInf, 0.f);
       }
+      return kNone;
     };
     // its Q rows: a thread takes one 16-byte column of every RS-th row (a whole number of tokens apart, since
     // the group divides RS), all loads in flight, then into the swizzled K-major layout
@@ -839,15 +856,15 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_ready[x]);
     };
-    bool have = advance();
-    if (have) {
+    int got = advance(true);
+    if (got == kHave) {
       uint4 u[QB];
       load_q(u);
       store_q(u);
       if (r == 0) *q_here = 1;
       q_arrive();
     }
-    while (have) {
+    while (got == kHave) {
       p = q;
       const Part t = tq;
       const Soft f{a, ls, p, t, smem, full, &s_full[x], &p_ready[x], &pv_done[x], both, armed, dead,
@@ -858,32 +875,31 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
       float m = kNegInf, l = 0.f;
       bool any = false;
       const bool tr = t.mode == kTransposed;
-      // the next piece is fetched and its Q rows are under way during this one's tiles, where a thread has
-      // registers for them
+      // its Q rows are under way during this one's tiles, where a thread has registers for them
       uint4 u[QB];
-      auto fetch = [&]() {
-        have = advance();
-        if (have) load_q(u);
+      auto fetch = [&](bool wait) {
+        got = advance(wait);
+        if (got == kHave) load_q(u);
       };
       if (!tr) {
         rows_tiles<DT, D>(f, nt, m, l, any);
-        fetch();
+        fetch(false);
       } else if (t.nr <= 8) {
-        fetch();
+        fetch(false);
         any = cols_tiles<DT, D, 8>(f, nt, ml);
       } else if (t.nr <= 16) {
-        fetch();
+        fetch(false);
         any = cols_tiles<DT, D, 16>(f, nt, ml);
       } else if (t.nr <= 32) {
-        fetch();
+        fetch(false);
         any = cols_tiles<DT, D, 32>(f, nt, ml);
       } else {
         any = cols_tiles<DT, D, 64>(f, nt, ml);
-        fetch();
+        fetch(false);
       }
       wait_bar(&pv_done[x], (nt - 1) & 1, dead, a.status);
       tc_fence_after();
-      if (have) {
+      if (got == kHave) {
         store_q(u);
         q_arrive();
       }
@@ -899,6 +915,13 @@ __global__ void __launch_bounds__(kMmaThreads, 1)
         if (r == 0) *f.poison = 0;
         if (t.mode == kHalf) f.meet();
         else named_sync(1 + x, 128);
+      }
+      if (got == kNone) {
+        fetch(true);
+        if (got == kHave) {
+          store_q(u);
+          q_arrive();
+        }
       }
     }
   }

@@ -272,6 +272,9 @@ CASES = [
     # a full row tile over many key tiles, then pages of one and of several key tiles in turn
     (32, 8, 128, 9000, 64, [(b * 397) % 900 if b % 3 else b for b in range(64)], [1] * 64),
     (16, 2, 64, 4100, 16, [(b * 211) % 600 if b % 4 else 0 for b in range(40)], [1 + b % 3 for b in range(40)]),
+    # tall causal row tiles, and behind them many pieces in a row that only one of two streams takes part in
+    (32, 8, 128, 40, 32, [0] * 16, [70, 20, 20, 20, 25, 3, 20, 20, 20, 100, 20, 31, 1, 20, 20, 65]),
+    (32, 8, 128, 3000, 16, [0] * 40, [97] + [20 + b % 12 for b in range(18)] + [1, 130] + [20] * 18 + [257]),
 ]
 
 

@@ -200,8 +200,9 @@ __global__ void __launch_bounds__(kPlanThreads) release_pages_kernel(PagePlanArg
   if (tid == 0) *a.n_free_out = n_free + total;
 }
 
-// One B200, a step of 64 tokens 5 us; 147 thousand tokens of 256 prompts see the token loop's width: 51 us on
-// 8 CTAs, PLAN_GRID_US on as many as a thousand tokens each fill (2.9 MB written).
+// One B200: a step of 64 tokens takes 5.2 us, 131 thousand tokens of 256 prompts 6.0 us on as many CTAs as a
+// thousand tokens each fill (2.7 MB written; 51 us on a cluster of 8). Both are launch, scan and two dependent
+// loads; the bytes are 0.4 us.
 cudaError_t launch_plan_pages(const PagePlanArgs& args, cudaStream_t stream) {
   PagePlanArgs a = args;
   a.in_place = a.lens == a.lens_out || a.n_free == a.n_free_out;
@@ -243,6 +244,8 @@ cudaError_t launch_release_pages(const PagePlanArgs& a, cudaStream_t stream) {
 // pair of 16-byte chunks (i, i + D/2) of its rows, so that a token's loads are all in flight while D/2
 // threads work out its angles. The angle is reduced in 64 bits (a 32-bit product is off by 0.008 rad at
 // position 131072); the rotation is done in 32 bits and rounded once.
+// One B200, 32/8 heads of 128 in bf16: 8.5 thousand tokens (209 MB) 41 us, 5.1 TB/s, 78 % of the measured copy
+// rate; 64 tokens 3.8 us.
 // ----------------------------------------------------------------------------------------
 constexpr int kAppThreads = 512;
 

@@ -110,6 +110,8 @@ def plan_pages(lens, new_lens, block_table, free_pages, n_free, page_size: int, 
     _vector("n_free", n_free, i32, 1, dev)
     if n_tokens < 0:
         raise ValueError(f"n_tokens must not be negative, not {n_tokens}")
+    if not 0 <= base_pos < 1 << 31:
+        raise ValueError(f"base_pos must be a 32-bit position, not {base_pos}")
     if out is None:
         out = PagePlan(torch.empty(n_seq + 1, dtype=i32, device=dev), torch.empty(n_tokens, dtype=i64, device=dev),
                        torch.empty(n_tokens, dtype=i32, device=dev), torch.empty(n_tokens, dtype=i64, device=dev),

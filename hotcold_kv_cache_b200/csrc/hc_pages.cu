@@ -257,74 +257,70 @@ __global__ void __launch_bounds__(kAppThreads) append_pages_kernel(PageAppendArg
   __shared__ float s_cos[H], s_sin[H];
   pdl_wait();
   const int t = blockIdx.x, tid = threadIdx.x;
+  const int nq = a.q_out ? a.Hq : 0, items = (nq + 2 * a.Hk) * CH;
+  // a pair of chunks: of a query head, of a key head, of a value head
+  auto source = [&](int x) {
+    const int hh = x / CH;
+    if (hh < nq) return reinterpret_cast<const T*>(a.q) + t * a.q_st + hh * a.q_sh;
+    if (hh < nq + a.Hk) return reinterpret_cast<const T*>(a.k) + t * a.k_st + (hh - nq) * a.k_sh;
+    return reinterpret_cast<const T*>(a.v) + t * a.v_st + (hh - nq - a.Hk) * a.v_sh;
+  };
+  // the rows, the slot and the position are read side by side
+  uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+  if (tid < items) {
+    const uint4* src = reinterpret_cast<const uint4*>(source(tid)) + tid % CH;
+    lo = src[0];
+    hi = src[CH];
+  }
   const int64_t slot = a.slots[t];
-  const int64_t pos = a.inv_freq && tid < H ? a.positions[t] : 0;
+  if (a.inv_freq && tid < H) {
+    const double ang = (double)a.inv_freq[tid] * (double)a.positions[t];
+    const double n = rint(ang * 0.15915494309189535);  // 1 / (2 pi)
+    // 2 pi as the nearest double and what that leaves
+    const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, ang));
+    float cs, sn;
+    sincosf((float)r, &sn, &cs);
+    s_cos[tid] = cs * a.rope_scaling;
+    s_sin[tid] = sn * a.rope_scaling;
+  }
+  __syncthreads();
   if (slot < 0 || slot >= (int64_t)a.n_pages * a.page_size) {
     if (slot != -1 && tid == 0 && a.status) atomicOr(a.status, HC_DEV_INDEX);
     return;
   }
-  const int64_t page = slot / a.page_size, row = slot % a.page_size;
-  const int nq = a.q_out ? a.Hq : 0, items = (nq + 2 * a.Hk) * CH;
-  bool first = true;
-  for (int x = tid; x - tid < items; x += blockDim.x) {
+  const int64_t page = slot >> (__ffs(a.page_size) - 1);
+  const int row = (int)slot & (a.page_size - 1);
+  for (int x = tid; x < items; x += blockDim.x) {
     const int hh = x / CH, c = x % CH;
-    const T* src = nullptr;
-    T* dst = nullptr;
-    bool turn = a.inv_freq != nullptr;
-    if (x < items) {
-      if (hh < nq) {
-        src = reinterpret_cast<const T*>(a.q) + t * a.q_st + hh * a.q_sh;
-        dst = reinterpret_cast<T*>(a.q_out) + ((size_t)t * a.Hq + hh) * D;
-      } else {
-        const int h = hh < nq + a.Hk ? hh - nq : hh - nq - a.Hk;
-        const size_t off = (((size_t)page * a.Hk + h) * a.page_size + row) * D;
-        if (hh < nq + a.Hk) {
-          src = reinterpret_cast<const T*>(a.k) + t * a.k_st + h * a.k_sh;
-          dst = reinterpret_cast<T*>(a.k_pages) + off;
-        } else {
-          src = reinterpret_cast<const T*>(a.v) + t * a.v_st + h * a.v_sh;
-          dst = reinterpret_cast<T*>(a.v_pages) + off;
-          turn = false;
-        }
-      }
+    if (x != tid) {
+      const uint4* src = reinterpret_cast<const uint4*>(source(x)) + c;
+      lo = src[0];
+      hi = src[CH];
     }
-    uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
-    if (src) {
-      lo = reinterpret_cast<const uint4*>(src)[c];
-      hi = reinterpret_cast<const uint4*>(src + H)[c];
+    T* dst;
+    if (hh < nq) {
+      dst = reinterpret_cast<T*>(a.q_out) + ((size_t)t * a.Hq + hh) * D;
+    } else {
+      const bool key = hh < nq + a.Hk;
+      const size_t off = (((size_t)page * a.Hk + hh - nq - (key ? 0 : a.Hk)) * a.page_size + row) * D;
+      dst = reinterpret_cast<T*>(key ? a.k_pages : a.v_pages) + off;
     }
-    if (first && a.inv_freq) {
-      if (tid < H) {
-        const double ang = (double)a.inv_freq[tid] * (double)pos;
-        const double n = rint(ang * 0.15915494309189535);  // 1 / (2 pi)
-        // 2 pi as the nearest double and what that leaves
-        const double r = fma(-n, 2.4492935982947064e-16, fma(-n, 6.283185307179586, ang));
-        float cs, sn;
-        sincosf((float)r, &sn, &cs);
-        s_cos[tid] = cs * a.rope_scaling;
-        s_sin[tid] = sn * a.rope_scaling;
-      }
-      __syncthreads();
-    }
-    first = false;
-    if (src) {
-      if (turn) {
-        float fl[VEC], fh[VEC];
-        unpack16<DT>(lo, fl);
-        unpack16<DT>(hi, fh);
-        alignas(16) T ol[VEC], oh[VEC];
+    if (a.inv_freq && hh < nq + a.Hk) {
+      float fl[VEC], fh[VEC];
+      unpack16<DT>(lo, fl);
+      unpack16<DT>(hi, fh);
+      alignas(16) T ol[VEC], oh[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float cs = s_cos[c * VEC + e], sn = s_sin[c * VEC + e];
-          ol[e] = E::from_f(fl[e] * cs - fh[e] * sn);
-          oh[e] = E::from_f(fh[e] * cs + fl[e] * sn);
-        }
-        lo = *reinterpret_cast<uint4*>(ol);
-        hi = *reinterpret_cast<uint4*>(oh);
+      for (int e = 0; e < VEC; ++e) {
+        const float cs = s_cos[c * VEC + e], sn = s_sin[c * VEC + e];
+        ol[e] = E::from_f(fl[e] * cs - fh[e] * sn);
+        oh[e] = E::from_f(fh[e] * cs + fl[e] * sn);
       }
-      reinterpret_cast<uint4*>(dst)[c] = lo;
-      reinterpret_cast<uint4*>(dst + H)[c] = hi;
+      lo = *reinterpret_cast<uint4*>(ol);
+      hi = *reinterpret_cast<uint4*>(oh);
     }
+    reinterpret_cast<uint4*>(dst)[c] = lo;
+    reinterpret_cast<uint4*>(dst + H)[c] = hi;
   }
 }
 

@@ -200,7 +200,7 @@ def append_pages(q, k, v, slots, positions, k_pages, v_pages, inv_freq=None, rop
             Hq = q.shape[1]
             q, qp, q_st, q_sh = _rows16(q)
             if q_out is None:
-                q_out = torch.empty((T, Hq, D), dtype=dtype, device=dev)
+                q_out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((T, Hq, D))
             else:
                 _check("q_out", q_out, dtype, (T, Hq, D), dev)
             qo = q_out.data_ptr()
@@ -261,7 +261,7 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k_pages, v_pages, block_table
         _vector("prefix_mask", prefix_mask, torch.uint8, P, dev)
     q, qp, q_st, q_sh = _rows16(q)
     if out is None:
-        out = torch.empty((T, Hq, D), dtype=dtype, device=dev)
+        out = torch.empty_like(q) if q.is_contiguous() else q.new_empty((T, Hq, D))
     else:
         _check("out", out, dtype, (T, Hq, D), dev)
     lse = torch.empty((T, Hq), dtype=torch.float32, device=dev) if return_lse else None
@@ -276,9 +276,10 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k_pages, v_pages, block_table
             if len(_SCRATCH_BYTES) < 4096:
                 _SCRATCH_BYTES[key] = nbytes
         # this call's own: two streams, or two captured graphs, never share it
-        scratch = torch.empty(max(nbytes, 16), dtype=torch.uint8, device=dev)
+        es = 4 if code == _lib.HC_F32 else 2
+        scratch = q.new_empty(nbytes // es + 8)
         _call("hc_shared_prefix_attention", dev, qp, q_st, q_sh, pk, ks0, ks1, pv, vs0, vs1, _lib.ptr(prefix_mask),
               k_pages.data_ptr(), v_pages.data_ptr(), block_table.data_ptr(), lens.data_ptr(), cu_new.data_ptr(),
               out.data_ptr(), _lib.ptr(lse), _lib.ptr(status), T, n_seq, Hq, Hk, D, P, page_size, max_blocks, n_pages,
-              code, scaling, scratch.data_ptr(), scratch.numel())
+              code, scaling, scratch.data_ptr(), scratch.numel() * es)
     return (out, lse) if return_lse else out

@@ -205,7 +205,7 @@ __global__ void __launch_bounds__(kPlanThreads) release_pages_kernel(PagePlanArg
 // loads; the bytes are 0.4 us.
 cudaError_t launch_plan_pages(const PagePlanArgs& args, cudaStream_t stream) {
   PagePlanArgs a = args;
-  a.in_place = a.lens == a.lens_out || a.n_free == a.n_free_out;
+  a.in_place = a.lens == a.lens_out || a.new_lens == a.lens_out || a.n_free == a.n_free_out;
   const int want = (int)(((int64_t)a.n_tokens + kPlanThreads - 1) / kPlanThreads);
   if (want > 16) {
     const int ctas = want / 2 < 296 ? want / 2 : 296;

@@ -387,8 +387,8 @@ HC_API int hc_splice_hits(const hc_layer* L, const int32_t* hit_ids, int k, void
  * block_table, lens_out = lens + new_lens, n_free_out = n_free - fresh pages, cu_new (n_seq + 1) is the
  * running sum of new_lens, and for each of the n_tokens rows t of the step: seq_ids the sequence,
  * slots = page * page_size + row in the page, positions = base_pos + place in the sequence; all three
- * are -1 behind the last token. lens_out / n_free_out may be lens / n_free (the step is committed) or
- * other buffers (it may be thrown away: the next plan writes over it). When the tokens exceed
+ * are -1 behind the last token. lens_out / n_free_out may be lens / n_free (the step is committed;
+ * lens_out may be new_lens too) or other buffers (it may be thrown away: the next plan writes over it). When the tokens exceed
  * n_tokens, the fresh pages n_free or a sequence max_blocks, or a length is negative or out of range,
  * nothing changes (lens_out = lens, no tokens, slots -1) and status gets HC_DEV_CAPACITY or HC_DEV_INDEX.
  *
@@ -426,8 +426,10 @@ HC_API int hc_append_pages(const void* q, int64_t q_st, int64_t q_sh, const void
  * once for the whole batch. out (T,Hq,D) contiguous; lse (T,Hq) fp32, or NULL: the natural log of the
  * sum of exponentials. A row that attends nothing is 0 with lse -inf; rows from cu_new[n_seq] on are
  * left as they were. A block table entry outside the pool reads as zero keys and values, a length
- * outside max_blocks pages is cut, and both set HC_DEV_INDEX. T <= 65536. Scratch from
- * hc_shared_prefix_attention_scratch_bytes, used by one call at a time.
+ * outside max_blocks pages is cut, and both set HC_DEV_INDEX; a wait inside the kernel that ran out
+ * sets HC_DEV_TIMEOUT, and the call's results are then worthless. T <= 65536. Scratch from
+ * hc_shared_prefix_attention_scratch_bytes (asked for with the call's device current: the work is
+ * divided among its multiprocessors), used by one call at a time.
  */
 HC_API size_t hc_shared_prefix_attention_scratch_bytes(int dtype, int T, int n_seq, int Hq, int Hk, int D, int P);
 HC_API int hc_shared_prefix_attention(const void* q, int64_t q_st, int64_t q_sh, const void* prefix_k, int64_t pk_sh,

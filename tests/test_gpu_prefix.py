@@ -74,6 +74,23 @@ def test_plan(n_seq, ps, ctx, new, pad, commit):
         assert np.array_equal(g["lens"].cpu().numpy(), c) and int(g["n_free"]) == n_free
 
 
+@pytest.mark.parametrize("n_seq,new", [(3, 5), (300, 400)])
+def test_plan_over_its_own_inputs(n_seq, new):
+    """The lengths after the step may go where the new lengths came from, for one CTA's step and for many."""
+    import hotcold_kv_cache_b200 as hc
+    rng = np.random.default_rng(n_seq)
+    c, a = rng.integers(0, 50, n_seq), rng.integers(0, new + 1, n_seq)
+    table, free, n_free = make_table(rng, c, 16, 40, 30 * n_seq)
+    want = R.plan(c, a, table, free, n_free, 16, int(a.sum()), 0)
+    add = dev(a, torch.int32)
+    out = spare_out(n_seq, int(a.sum()))._replace(lens=add)
+    nf = dev([n_free], torch.int32)
+    p = hc.plan_pages(dev(c, torch.int32), add, dev(table, torch.int32), dev(free, torch.int32), nf, 16, int(a.sum()), out=out)
+    for name in ("cu_new", "slots", "seq_ids", "positions", "lens"):
+        assert np.array_equal(getattr(p, name).cpu().numpy(), want[name]), name
+    assert int(p.n_free) == want["n_free"] and int(nf) == n_free and int(p.status) == 0
+
+
 @pytest.mark.parametrize("what,bit", [("pages", CAPACITY), ("rows", CAPACITY), ("table", CAPACITY),
                                       ("negative_new", INDEX), ("negative_len", INDEX), ("long_len", INDEX),
                                       ("n_free", INDEX)])

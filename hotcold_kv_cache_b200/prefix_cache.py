@@ -100,7 +100,7 @@ class SharedPrefixCache(Cache):
             ok = x.stride(2) == 1 and x.stride(0) % per == 0 and x.stride(1) % per == 0 and x.data_ptr() % 16 == 0
             return x if ok and x.stride(0) > 0 and x.stride(1) > 0 else x.contiguous()
 
-        layer.prefix_k, layer.prefix_v = rows(k), rows(v)
+        layer.prefix_k, layer.prefix_v = rows(k.detach()), rows(v.detach())
         layer.is_initialized = True
         self.prefix_len = int(k.shape[1])
 
@@ -139,16 +139,22 @@ class SharedPrefixCache(Cache):
     def next_lens(self, lens: Sequence[int]):
         """How many of the next forward's tokens of each row are real (the row's first ones; the rest is
         padding, whose outputs mean nothing). Without it all are."""
+        self._begun("next_lens")
         lens = [int(x) for x in lens]
         if len(lens) != self.n_seq or min(lens) < 0:
             raise ValueError(f"next_lens needs {self.n_seq} lengths, none negative")
         self._next = lens
+
+    def _begun(self, name: str):
+        if self.n_seq == 0:
+            raise RuntimeError(f"{name} comes after begin()")
 
     def _pages(self, lens) -> int:
         return sum(-(-x // self.page_size) for x in lens)
 
     def start_step(self, batch: int, tokens: int):
         """Page plan of a forward of (batch, tokens), shared by its layers."""
+        self._begun("a step")
         if batch != self.n_seq:
             raise ValueError(f"the batch has {batch} rows, the cache {self.n_seq} sequences")
         new = self._next if self._next is not None else [tokens] * self.n_seq
@@ -192,6 +198,7 @@ class SharedPrefixCache(Cache):
 
     def release(self, keep_lens: Sequence[int]):
         """Sequence b keeps its first keep_lens[b] own tokens (0 frees it for another request)."""
+        self._begun("release")
         keep = [int(x) for x in keep_lens]
         if len(keep) != self.n_seq or any(x < 0 or x > n for x, n in zip(keep, self.host_lens)):
             raise ValueError(f"release keeps {keep} of {self.host_lens} tokens")
@@ -201,7 +208,30 @@ class SharedPrefixCache(Cache):
 
     def device_status(self) -> int:
         """OR of the HC_DEV_* bits of the steps so far (synchronises)."""
+        if self.n_seq == 0:
+            return 0
         return int(self.status) | (int(self.plan.status) if self.plan is not None else 0)
+
+    # ------------------------------------------------------------------ what transformers may ask of a cache
+    # Its own versions work on dense keys and values of a layer, here the prefix of all sequences.
+    def _refuse(self, name: str):
+        raise NotImplementedError(f"a shared-prefix cache has no {name}: sequences are cut or freed with release(), "
+                                  "another document takes another cache")
+
+    def reset(self):
+        self._refuse("reset")
+
+    def crop(self, max_length):
+        self._refuse("crop")
+
+    def reorder_cache(self, beam_idx):
+        self._refuse("reorder_cache (beam search)")
+
+    def batch_repeat_interleave(self, repeats):
+        self._refuse("batch_repeat_interleave")
+
+    def batch_select_indices(self, indices):
+        self._refuse("batch_select_indices")
 
 
 def build_shared_prefix_cache(model, page_size: int = 64) -> SharedPrefixCache:

@@ -81,3 +81,37 @@ def test_plain_plan():
     assert r["positions"][:2].tolist() == [115, 116] and r["n_free"] == 2
     assert r["table"].tolist() == [[4, 3, -1], [2, -1, -1]]
     assert R.plan([15, 0], [2, 16], table, np.array([0]), 1, 16, 18, 0) is None
+
+
+def cpu_cache(n_layers=2):
+    from hotcold_kv_cache_b200.prefix_cache import SharedPrefixCache
+    cache, k = SharedPrefixCache(n_layers, torch.ones(32)), torch.randn(2, 8, 64)
+    for i in range(n_layers):
+        cache.set_prefix(i, k.clone(), k.clone())
+    return cache, k
+
+
+def test_cache_refuses_what_it_cannot_do():
+    """Beam reordering, cropping and resetting would touch the prefix or leave the pages as they were."""
+    cache, k = cpu_cache()
+    one = torch.tensor([0])
+    for name, args in [("reset", ()), ("crop", (3,)), ("reorder_cache", (one,)), ("batch_repeat_interleave", (2,)),
+                       ("batch_select_indices", (one,))]:
+        with pytest.raises(NotImplementedError, match=name):
+            getattr(cache, name)(*args)
+    assert all(torch.equal(x.prefix_k, k) and torch.equal(x.prefix_v, k) for x in cache.layers)
+
+
+def test_cache_before_begin():
+    cache, _ = cpu_cache()
+    for call in (lambda: cache.release([]), lambda: cache.next_lens([]), lambda: cache.start_step(1, 1)):
+        with pytest.raises(RuntimeError, match="begin"):
+            call()
+    assert cache.device_status() == 0
+
+
+def test_cache_keeps_no_autograd_graph():
+    from hotcold_kv_cache_b200.prefix_cache import SharedPrefixCache
+    cache, k = SharedPrefixCache(1, torch.ones(32)), torch.randn(2, 8, 64, requires_grad=True)
+    cache.set_prefix(0, k * 2, k * 3)
+    assert not cache.layers[0].prefix_k.requires_grad and not cache.layers[0].prefix_v.requires_grad

@@ -145,6 +145,12 @@ class SharedPrefixCache(Cache):
             raise ValueError(f"next_lens needs {self.n_seq} lengths, none negative")
         self._next = lens
 
+    def refresh_lens(self):
+        """Read the sequences' lengths back from the device (synchronises): replays of a captured step advance
+        them there only, and the checks of later steps and release() go by the host's."""
+        self._begun("refresh_lens")
+        self.host_lens = self.lens.tolist()
+
     def _begun(self, name: str):
         if self.n_seq == 0:
             raise RuntimeError(f"{name} comes after begin()")
@@ -241,9 +247,20 @@ def build_shared_prefix_cache(model, page_size: int = 64) -> SharedPrefixCache:
                              page_size)
 
 
+def hides_keys(mask: Optional[torch.Tensor]) -> bool:
+    """Whether an attention mask (B, 1, T, keys), bool or additive, hides a key from a sequence's last row, which a
+    causal mask alone shows everything. Synchronises; under capture, where that cannot be, it says no."""
+    if mask is None or mask.dim() != 4 or (mask.is_cuda and torch.cuda.is_current_stream_capturing()):
+        return False
+    last = mask[:, :, -1]
+    return not bool((last if mask.dtype is torch.bool else last == 0).all())
+
+
 def shared_prefix_forward(attn, hidden_states, position_embeddings, attention_mask, cache: SharedPrefixCache):
     """LlamaAttention.forward over a SharedPrefixCache: before begin() the prefix's forward (transformers' RoPE and
-    stock causal attention, as the patched prompt forward), after it the batch's step."""
+    stock causal attention, as the patched prompt forward), after it the batch's step, whose positions and mask
+    are the cache's own: padding comes from next_lens(). A mask that hides keys from a step of several tokens is
+    refused where next_lens() says nothing."""
     from transformers.models.llama import modeling_llama
     b, t, _ = hidden_states.shape
     li, d = int(attn.layer_idx), int(attn.head_dim)
@@ -263,6 +280,9 @@ def shared_prefix_forward(attn, hidden_states, position_embeddings, attention_ma
                                              is_causal=attention_mask is None and t > 1)
         return attn.o_proj(out.transpose(1, 2).reshape(b, t, -1)), None
     if li == 0:
+        if t > 1 and cache._next is None and hides_keys(attention_mask):
+            raise ValueError("the attention mask hides keys of a step: name its padding with next_lens(), and the prefix's "
+                             "with begin(prefix_mask=); a shared-prefix cache does not read the mask")
         cache.start_step(b, t)
     out = cache.attend(li, q.reshape(b * t, -1, d), k.reshape(b * t, -1, d), v.reshape(b * t, -1, d), float(attn.scaling))
     return attn.o_proj(out.reshape(b, t, -1)), None

@@ -153,3 +153,79 @@ def test_refusals():
         hc.uninstall_monkeypatch()
     with pytest.raises(ValueError):
         hc.build_shared_prefix_cache(model, page_size=24)
+
+
+def test_padding_comes_from_next_lens():
+    """A padded batch's attention mask is refused, or the step is told its padding and the mask is not needed."""
+    import hotcold_kv_cache_b200 as hc
+    model, ids = setup(torch.float16)
+    prefix, q = ids(1, 40), ids(2, 6)
+    full = torch.ones(2, 46, dtype=torch.long, device="cuda")
+    padded = full.clone()
+    padded[1, 44:] = 0
+    hc.install_monkeypatch(enable_debug=False)
+    try:
+        with torch.inference_mode():
+            def begun():
+                cache = hc.build_shared_prefix_cache(model, page_size=16)
+                model(input_ids=prefix, past_key_values=cache, use_cache=True)
+                cache.begin(2, max_new_tokens=16)
+                return cache
+
+            cache = begun()
+            with pytest.raises(ValueError, match="next_lens"):
+                model(input_ids=q, attention_mask=padded, past_key_values=cache, use_cache=True)
+            assert cache.host_lens == [0, 0] and cache.lens.tolist() == [0, 0]
+            a = model(input_ids=q, attention_mask=full, past_key_values=cache, use_cache=True).logits
+            cache = begun()
+            assert torch.equal(a, model(input_ids=q, past_key_values=cache, use_cache=True).logits)
+            cache = begun()
+            cache.next_lens([6, 4])
+            b = model(input_ids=q, attention_mask=padded, past_key_values=cache, use_cache=True).logits
+            cache = begun()
+            cache.next_lens([6, 4])
+            c = model(input_ids=q, past_key_values=cache, use_cache=True).logits
+            assert torch.equal(b[0], c[0]) and torch.equal(b[1, :4], c[1, :4]) and cache.device_status() == 0
+    finally:
+        hc.uninstall_monkeypatch()
+
+
+def test_lengths_after_replays():
+    """Replays advance the lengths on the device; refresh_lens brings the host's up, and steps go on from there."""
+    import hotcold_kv_cache_b200 as hc
+    model, ids = setup(torch.float16)
+    prefix, q, steps = ids(1, 40), ids(2, 5), [ids(2, 1) for _ in range(3)]
+    hc.install_monkeypatch(enable_debug=False)
+    try:
+        with torch.inference_mode():
+            def run(graph):
+                cache = hc.build_shared_prefix_cache(model, page_size=16)
+                model(input_ids=prefix, past_key_values=cache, use_cache=True)
+                cache.begin(2, max_new_tokens=16)
+                model(input_ids=q, past_key_values=cache, use_cache=True)
+                tok = steps[0].clone()
+                if graph:
+                    side = torch.cuda.Stream()
+                    side.wait_stream(torch.cuda.current_stream())
+                    with torch.cuda.stream(side):
+                        model(input_ids=tok, past_key_values=cache, use_cache=True)
+                        cache.release([5, 5])
+                    torch.cuda.current_stream().wait_stream(side)
+                    g = torch.cuda.CUDAGraph()
+                    with torch.cuda.graph(g):
+                        model(input_ids=tok, past_key_values=cache, use_cache=True)
+                    for s in steps[:2]:
+                        tok.copy_(s)
+                        g.replay()
+                    cache.refresh_lens()
+                else:
+                    for s in steps[:2]:
+                        model(input_ids=s, past_key_values=cache, use_cache=True)
+                assert cache.host_lens == [7, 7] and cache.get_seq_length() == 47
+                cache.release([7, 6])
+                out = model(input_ids=steps[2], past_key_values=cache, use_cache=True).logits
+                assert cache.host_lens == cache.lens.tolist() == [8, 7] and cache.device_status() == 0
+                return out
+            assert torch.equal(run(True), run(False))
+    finally:
+        hc.uninstall_monkeypatch()

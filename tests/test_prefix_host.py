@@ -115,3 +115,16 @@ def test_cache_keeps_no_autograd_graph():
     cache, k = SharedPrefixCache(1, torch.ones(32)), torch.randn(2, 8, 64, requires_grad=True)
     cache.set_prefix(0, k * 2, k * 3)
     assert not cache.layers[0].prefix_k.requires_grad and not cache.layers[0].prefix_v.requires_grad
+
+
+@pytest.mark.parametrize("hidden", [None, (0, 0), (1, 5), (1, 6)])
+@pytest.mark.parametrize("dtype", [torch.bool, torch.float32, torch.bfloat16])
+def test_hidden_keys_of_a_mask(dtype, hidden):
+    """A causal mask of 3 tokens behind 4 hides nothing; one padded on the left or the right does."""
+    from hotcold_kv_cache_b200.prefix_cache import hides_keys
+    see = torch.ones(3, 7, dtype=torch.bool).tril(4).expand(2, 1, 3, 7).clone()
+    if hidden is not None:
+        see[hidden[0], :, :, hidden[1]] = False
+    mask = see if dtype is torch.bool else torch.zeros(see.shape, dtype=dtype).masked_fill(~see, torch.finfo(dtype).min)
+    assert hides_keys(mask) is (hidden is not None)
+    assert not hides_keys(None)

@@ -94,7 +94,7 @@ def plan_pages(lens, new_lens, block_table, free_pages, n_free, page_size: int, 
     the sum of new_lens; rows behind the last token get -1), base_pos the position of a sequence's first
     token (the prefix length). Without `out` the step is committed: lens and n_free are updated in place
     and returned in the plan. With `out`, the plan goes into its tensors; out.lens and out.n_free may be
-    lens and n_free themselves (commit) or others (the step may be thrown away: the next plan starts from
+    lens and n_free themselves (commit; out.lens may be new_lens too) or others (the step may be thrown away: the next plan starts from
     the same state). When the tokens do not fit n_tokens, the free pages or the tables, nothing is
     changed, the plan has no tokens and status gets HC_DEV_CAPACITY; a length out of range likewise with
     HC_DEV_INDEX."""
@@ -178,7 +178,8 @@ def append_pages(q, k, v, slots, positions, k_pages, v_pages, inv_freq=None, rop
     (i, i + D/2) is positions[t] * inv_freq[i] (inv_freq (D/2) float32), cos and sin times rope_scaling,
     rounded once; without inv_freq q and k are taken as rotated and q is returned as it is. Returns the
     rotated queries (q_out when given, (T,Hq,D) contiguous). Tokens with slot -1 are skipped and their
-    rows of q_out left alone; another slot outside the pool sets HC_DEV_INDEX in status (1) int32."""
+    rows of q_out left alone; another slot outside the pool sets HC_DEV_INDEX in status (1) int32. Of two
+    tokens with the same slot either one's keys and values stay, in parts too: plan_pages never makes any."""
     dev = _cuda("k", k)
     T, Hk, D = k.shape
     dtype = k.dtype

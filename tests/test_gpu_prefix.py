@@ -544,3 +544,18 @@ def test_refusals():
         hc.append_pages(k, k, k, z.int(), z, s["k_pages"], s["v_pages"])
     with pytest.raises(ValueError):
         hc.append_pages(k, k, k, z, z, s["k_pages"], s["v_pages"], q_out=k)
+
+
+@pytest.mark.parametrize("base,ok", [(-1, False), (1 << 31, False), ((1 << 31) - 1, True)])
+def test_base_position_bounds(base, ok):
+    """Positions are 64 bits, their base 32: the last one that fits is taken, the next refused."""
+    import hotcold_kv_cache_b200 as hc
+    args = (dev([3], torch.int32), dev([2], torch.int32), dev([[0]], torch.int32), dev([0], torch.int32),
+            dev([0], torch.int32), 16, 2)
+    if not ok:
+        with pytest.raises(ValueError, match="base_pos"):
+            hc.plan_pages(*args, base_pos=base)
+        assert args[0].tolist() == [3]
+        return
+    p = hc.plan_pages(*args, base_pos=base)
+    assert p.positions.tolist() == [base + 3, base + 4] and p.slots.tolist() == [3, 4] and int(p.status) == 0

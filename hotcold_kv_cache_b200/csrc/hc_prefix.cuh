@@ -105,9 +105,9 @@ __device__ __forceinline__ int seq_keys(const SeqLens& s, int tok1) {  // keys s
 
 // Quotient of line positions: 64-bit division, out of the way, only where 32 bits do not hold them (a kernel
 // starts with cold instruction caches, and its first microseconds are fetches of what it runs through).
-static __device__ __noinline__ int line_div64(int64_t x, int64_t y) { return (int)(x / y); }
-__device__ __forceinline__ int line_div(int64_t x, int64_t y) {
-  return (x | y) >> 32 ? line_div64(x, y) : (int)((uint32_t)x / (uint32_t)y);
+static __device__ __noinline__ int64_t line_div64(int64_t x, int64_t y) { return x / y; }
+__device__ __forceinline__ int line_div(int64_t x, int64_t y) {  // numbers of CTAs, groups or tiles: 32 bits hold them
+  return (x | y) >> 32 ? (int)line_div64(x, y) : (int)((uint32_t)x / (uint32_t)y);
 }
 
 struct LineGeom {
@@ -171,7 +171,9 @@ __device__ __forceinline__ Stretch line_setup(const PrefixArgs& a, const LineSha
   before += x - mine + g.vpre;
   total += g.vpre;
   Stretch r;
-  r.W = max((int64_t)line_div(total + s.nc - 1, s.nc), (int64_t)min_stretch(s));
+  // a stretch may pass 32 bits: 65536 tokens of one sequence over 2^30 keys are 4.6e9 long
+  const int64_t up = total + s.nc - 1;
+  r.W = max(up >> 32 ? line_div64(up, s.nc) : (int64_t)((uint32_t)up / (uint32_t)s.nc), (int64_t)min_stretch(s));
   r.v = min(c * r.W, total);
   r.v_end = min((c + 1) * r.W, total);
   if (c == 0 && tid == 0) hdr[0] = r.W;

@@ -72,11 +72,14 @@ class SharedPrefixLayer(CacheLayerMixin):
 
 
 class SharedPrefixCache(Cache):
-    def __init__(self, n_layers: int, inv_freq: torch.Tensor, rope_scaling: float = 1.0, page_size: int = 64):
+    """`rotary`: a rotary module whose inv_freq and attention_scaling take the place of the two given here. They are
+    read in begin() and at every step, since a module whose frequencies follow the length replaces them in a forward."""
+
+    def __init__(self, n_layers: int, inv_freq: torch.Tensor, rope_scaling: float = 1.0, page_size: int = 64, rotary=None):
         if page_size < 16 or page_size > 256 or page_size & (page_size - 1):
             raise ValueError(f"page_size must be a power of two from 16 to 256, not {page_size}")
         super().__init__(layers=[SharedPrefixLayer(self, i) for i in range(n_layers)])
-        self.inv_freq, self.rope_scaling, self.page_size = inv_freq, float(rope_scaling), int(page_size)
+        self.inv_freq, self.rope_scaling, self.page_size, self.rotary = inv_freq, float(rope_scaling), int(page_size), rotary
         self.prefix_len = 0
         self.prefix_mask: Optional[torch.Tensor] = None
         self.n_seq = 0  # 0 until begin()
@@ -126,7 +129,7 @@ class SharedPrefixCache(Cache):
         self.n_free = torch.full((1,), self.n_pages, **z)
         self.status = torch.zeros(1, **z)
         self.prefix_mask = None if prefix_mask is None else prefix_mask.to(device=dev, dtype=torch.uint8).contiguous()
-        self.inv_freq = self.inv_freq.detach().to(device=dev, dtype=torch.float32).contiguous()
+        self._read_rotary(dev)
         for layer in self.layers:
             if layer.prefix_k is None:
                 raise RuntimeError("begin() comes after the prefix's forward")
@@ -134,6 +137,12 @@ class SharedPrefixCache(Cache):
             layer.v_pages = torch.empty_like(layer.k_pages)
         self.host_lens = [0] * self.n_seq
         self._next = self.plan = None
+
+    def _read_rotary(self, dev):
+        """The frequencies and the factor on cos and sin that this forward's positions were turned by."""
+        if self.rotary is not None:
+            self.inv_freq, self.rope_scaling = self.rotary.inv_freq, float(getattr(self.rotary, "attention_scaling", 1.0))
+        self.inv_freq = self.inv_freq.detach().to(device=dev, dtype=torch.float32).contiguous()
 
     # ------------------------------------------------------------------ steps
     def next_lens(self, lens: Sequence[int]):
@@ -171,6 +180,7 @@ class SharedPrefixCache(Cache):
             raise RuntimeError(f"the pages do not hold this step: {self._pages(after)} of {self.n_pages} pages, longest "
                                f"sequence {max(after)} of {self.max_blocks * self.page_size} tokens")
         dev = self.lens.device
+        self._read_rotary(dev)
         n = batch * tokens
         uniform = min(new) == tokens
         add = torch.full((self.n_seq,), tokens, dtype=torch.int32, device=dev) if uniform else \
@@ -241,10 +251,9 @@ class SharedPrefixCache(Cache):
 
 
 def build_shared_prefix_cache(model, page_size: int = 64) -> SharedPrefixCache:
-    """A SharedPrefixCache for a Llama model: its layer count and rotary parameters."""
+    """A SharedPrefixCache for a Llama model: its layer count and rotary module."""
     rot = model.model.rotary_emb
-    return SharedPrefixCache(int(model.config.num_hidden_layers), rot.inv_freq, float(getattr(rot, "attention_scaling", 1.0)),
-                             page_size)
+    return SharedPrefixCache(int(model.config.num_hidden_layers), rot.inv_freq, page_size=page_size, rotary=rot)
 
 
 def hides_keys(mask: Optional[torch.Tensor]) -> bool:

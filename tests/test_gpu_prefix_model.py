@@ -229,3 +229,46 @@ def test_lengths_after_replays():
             assert torch.equal(run(True), run(False))
     finally:
         hc.uninstall_monkeypatch()
+
+
+@pytest.mark.parametrize("kind", ["dynamic", "longrope"])
+def test_rotary_that_follows_the_length(kind):
+    """Frequencies that move with the length: the steps turn by the frequencies of their own forward, as the stock model
+    does with a cache of the whole batch."""
+    import hotcold_kv_cache_b200 as hc
+    from transformers import DynamicCache, LlamaConfig, LlamaForCausalLM
+    rope = dict(rope_type="dynamic", factor=4.0, rope_theta=500000.0) if kind == "dynamic" else \
+        dict(rope_type="longrope", rope_theta=500000.0, factor=8.0, short_factor=[1.0] * 32,
+             long_factor=[1.0 + 0.1 * i for i in range(32)], original_max_position_embeddings=128)
+    cfg = {k: v for k, v in CFG.items() if k != "rope_theta"}
+    cfg["max_position_embeddings"] = 128
+
+    def fresh():  # the module keeps what a forward made of its frequencies
+        torch.manual_seed(5)
+        return LlamaForCausalLM(LlamaConfig(**cfg, rope_parameters=rope)).eval().cuda()
+
+    g = torch.Generator().manual_seed(6)
+    ids = lambda *s: torch.randint(0, CFG["vocab_size"], s, generator=g).cuda()  # noqa: E731
+    prefix, B = ids(1, 300), 2
+    steps = [ids(B, 9), ids(B, 1), ids(B, 70), ids(B, 1)]
+
+    def run(model, cache, first, begin):
+        model(input_ids=first, past_key_values=cache, use_cache=True)
+        if begin:
+            cache.begin(B, max_new_tokens=128)
+        return torch.cat([model(input_ids=s, past_key_values=cache, use_cache=True).logits for s in steps], 1)
+
+    with torch.inference_mode():
+        model = fresh()
+        before = model.model.rotary_emb.inv_freq.clone()
+        ref = run(model, DynamicCache(), prefix.expand(B, -1), False)
+        assert not torch.equal(model.model.rotary_emb.inv_freq, before)
+        model = fresh()
+        hc.install_monkeypatch(enable_debug=False)
+        try:
+            cache = hc.build_shared_prefix_cache(model, page_size=16)
+            got = run(model, cache, prefix, True)
+            assert cache.device_status() == 0
+        finally:
+            hc.uninstall_monkeypatch()
+    assert (got - ref).abs().max() <= TOL[torch.float32] * ref.abs().max()

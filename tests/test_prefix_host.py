@@ -128,3 +128,47 @@ def test_hidden_keys_of_a_mask(dtype, hidden):
     mask = see if dtype is torch.bool else torch.zeros(see.shape, dtype=dtype).masked_fill(~see, torch.finfo(dtype).min)
     assert hides_keys(mask) is (hidden is not None)
     assert not hides_keys(None)
+
+
+def cpu_model(rope=None, **kw):
+    from transformers import LlamaConfig, LlamaForCausalLM
+    torch.manual_seed(0)
+    more = {} if rope is None else dict(rope_parameters=rope)
+    return LlamaForCausalLM(LlamaConfig(vocab_size=50, hidden_size=128, intermediate_size=64, num_hidden_layers=2,
+                                        num_attention_heads=2, num_key_value_heads=1, head_dim=64,
+                                        max_position_embeddings=64, **more), **kw).eval()
+
+
+@pytest.fixture
+def patched():
+    import hotcold_kv_cache_b200 as hc
+    hc.install_monkeypatch(enable_debug=False)
+    yield hc
+    hc.uninstall_monkeypatch()
+
+
+ROPES = [dict(rope_type="dynamic", factor=2.0, rope_theta=10000.0),
+         dict(rope_type="longrope", rope_theta=10000.0, factor=4.0, short_factor=[1.0] * 32, long_factor=[2.0] * 32,
+              original_max_position_embeddings=64),
+         dict(rope_type="default", rope_theta=10000.0)]
+
+
+@pytest.mark.parametrize("rope", ROPES, ids=lambda r: r["rope_type"])
+def test_frequencies_are_the_model_s_own_now(patched, rope):
+    """A rotary module may replace its frequencies in the forward that passes its length: begin() and every step take
+    those of that forward, not those of the day the cache was built."""
+    model = cpu_model(rope)
+    rot = model.model.rotary_emb
+    with torch.no_grad():
+        cache = patched.build_shared_prefix_cache(model, page_size=16)
+        built = rot.inv_freq.clone()
+        model(input_ids=torch.randint(0, 50, (1, 200)), past_key_values=cache)
+        assert torch.equal(rot.inv_freq, built) is (rope["rope_type"] == "default")
+        cache.begin(2, 512)
+        assert torch.equal(cache.inv_freq, rot.inv_freq) and cache.rope_scaling == rot.attention_scaling
+        x = torch.zeros(1, 1, 128)
+        rot(x, torch.arange(700)[None])  # as the forward of a step that gets as far
+        rot.attention_scaling = 0.5
+        with pytest.raises(ValueError, match="CUDA"):  # the step itself needs a GPU
+            cache.start_step(2, 3)
+        assert torch.equal(cache.inv_freq, rot.inv_freq) and cache.rope_scaling == 0.5

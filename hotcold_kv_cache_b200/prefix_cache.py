@@ -256,11 +256,18 @@ def build_shared_prefix_cache(model, page_size: int = 64) -> SharedPrefixCache:
     return SharedPrefixCache(int(model.config.num_hidden_layers), rot.inv_freq, page_size=page_size, rotary=rot)
 
 
-def hides_keys(mask: Optional[torch.Tensor]) -> bool:
-    """Whether an attention mask (B, 1, T, keys), bool or additive, hides a key from a sequence's last row, which a
-    causal mask alone shows everything. Synchronises; under capture, where that cannot be, it says no."""
-    if mask is None or mask.dim() != 4 or (mask.is_cuda and torch.cuda.is_current_stream_capturing()):
+def hides_keys(mask) -> bool:
+    """Whether an attention mask hides a key: a (B, 1, T, keys) one, bool or additive, from a sequence's last row, which
+    a causal mask alone shows everything; a (B, keys) one, as flash attention is given, anywhere. Of another kind it
+    cannot tell and says yes. Synchronises; under capture, where that cannot be, it says no to the kinds it knows."""
+    if mask is None:
         return False
+    if not isinstance(mask, torch.Tensor) or mask.dim() not in (2, 4):
+        return True
+    if mask.is_cuda and torch.cuda.is_current_stream_capturing():
+        return False
+    if mask.dim() == 2:  # 1 or True: there
+        return not bool((mask != 0).all())
     last = mask[:, :, -1]
     return not bool((last if mask.dtype is torch.bool else last == 0).all())
 
@@ -281,6 +288,11 @@ def shared_prefix_forward(attn, hidden_states, position_embeddings, attention_ma
             raise ValueError("the prefix goes through the model as one sequence; begin() then opens the batch")
         qt, kt, vt = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
         cos, sin = position_embeddings
+        if attention_mask is not None and not (isinstance(attention_mask, torch.Tensor) and attention_mask.dim() == 4):
+            if hides_keys(attention_mask):
+                raise ValueError("the prefix's attention mask hides keys or is of a kind that is not read: hand the document in "
+                                 "without padding")
+            attention_mask = None  # a (1, P) mask of ones says nothing that is not causal
         qt, kt = modeling_llama.apply_rotary_pos_emb(qt, kt, cos, sin)
         cache.set_prefix(li, kt[0], vt[0])
         rep = qt.shape[1] // kt.shape[1]

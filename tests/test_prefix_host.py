@@ -172,3 +172,53 @@ def test_frequencies_are_the_model_s_own_now(patched, rope):
         with pytest.raises(ValueError, match="CUDA"):  # the step itself needs a GPU
             cache.start_step(2, 3)
         assert torch.equal(cache.inv_freq, rot.inv_freq) and cache.rope_scaling == 0.5
+
+
+@pytest.mark.parametrize("dtype", [torch.bool, torch.int64, torch.float32])
+def test_hidden_keys_of_a_flat_mask(dtype):
+    """A (B, keys) mask, as flash attention is given, hides where it is 0; of a kind not known nothing can be told."""
+    from hotcold_kv_cache_b200.prefix_cache import hides_keys
+    mask = torch.ones(2, 26).to(dtype)
+    assert not hides_keys(mask)
+    mask[1, 24:] = 0
+    assert hides_keys(mask)
+    assert hides_keys(mask[None]) and hides_keys(object())
+
+
+@pytest.mark.parametrize("kind", ["sdpa", "eager", "flash_attention_2"])
+@pytest.mark.parametrize("side", ["left", "right"])
+def test_padded_batch_is_refused_whatever_the_attention(patched, kind, side):
+    """The padding mask reaches the layers in the form of the model's attention implementation: each is refused."""
+    model = cpu_model()
+    model.config._attn_implementation = kind
+    with torch.no_grad():
+        cache = patched.build_shared_prefix_cache(model, page_size=16)
+        model(input_ids=torch.randint(0, 50, (1, 20)), past_key_values=cache)
+        cache.begin(2, 64)
+        mask = torch.ones(2, 26, dtype=torch.long)
+        mask[1, 24:] = 0
+        if side == "left":
+            mask[1] = mask[1].flip(0)
+        with pytest.raises(ValueError, match="next_lens"):
+            model(input_ids=torch.randint(0, 50, (2, 6)), attention_mask=mask, past_key_values=cache)
+        assert cache.host_lens == [0, 0] and cache.plan is None
+
+
+@pytest.mark.parametrize("kind", ["sdpa", "flash_attention_2"])
+def test_prefix_s_forward_under_either_mask(patched, kind):
+    """The prefix's forward is causal whatever form its mask has; a padded document is refused where its mask is flat."""
+    ids = torch.randint(0, 50, (1, 20))
+    model = cpu_model()
+    with torch.no_grad():
+        want = model(input_ids=ids, use_cache=False).logits
+        model.config._attn_implementation = kind
+        for mask in (None, torch.ones(1, 20, dtype=torch.long)):
+            cache = patched.build_shared_prefix_cache(model, page_size=16)
+            got = model(input_ids=ids, attention_mask=mask, past_key_values=cache).logits
+            assert (got - want).abs().max() <= 1e-5 * want.abs().max()
+        if kind == "flash_attention_2":
+            mask[0, 17:] = 0
+            cache = patched.build_shared_prefix_cache(model, page_size=16)
+            with pytest.raises(ValueError, match="padding"):
+                model(input_ids=ids, attention_mask=mask, past_key_values=cache)
+            assert cache.layers[0].prefix_k is None

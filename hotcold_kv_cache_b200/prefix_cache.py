@@ -82,6 +82,7 @@ class SharedPrefixCache(Cache):
         self.inv_freq, self.rope_scaling, self.page_size, self.rotary = inv_freq, float(rope_scaling), int(page_size), rotary
         self.prefix_len = 0
         self.prefix_mask: Optional[torch.Tensor] = None
+        self.prefix_hidden = False  # the prefix's forward had a mask that hides some of its tokens
         self.n_seq = 0  # 0 until begin()
         self.host_lens: List[int] = []  # own tokens of each sequence, as the device's lens
         self.plan: Optional[PagePlan] = None
@@ -111,10 +112,12 @@ class SharedPrefixCache(Cache):
               prefix_mask: Optional[torch.Tensor] = None):
         """n_seq empty sequences behind the prefix, each with at most max_new_tokens own tokens; the pages of
         all hold pool_tokens (default: enough for every sequence's most). prefix_mask (P) bool leaves prefix
-        tokens out."""
+        tokens out; a prefix that was padded needs it."""
         first = self.layers[0]
         if first.prefix_k is None:
             raise RuntimeError("begin() comes after the prefix's forward")
+        if self.prefix_hidden and prefix_mask is None:
+            raise ValueError("the prefix's attention mask hid some of its tokens: begin(prefix_mask=) says which stay hidden")
         if n_seq < 1 or max_new_tokens < 1:
             raise ValueError("begin() needs at least one sequence and one new token")
         dev, (Hk, _, D) = first.prefix_k.device, first.prefix_k.shape
@@ -295,6 +298,8 @@ def shared_prefix_forward(attn, hidden_states, position_embeddings, attention_ma
             attention_mask = None  # a (1, P) mask of ones says nothing that is not causal
         qt, kt = modeling_llama.apply_rotary_pos_emb(qt, kt, cos, sin)
         cache.set_prefix(li, kt[0], vt[0])
+        if li == 0:
+            cache.prefix_hidden = hides_keys(attention_mask)
         rep = qt.shape[1] // kt.shape[1]
         kr, vr = (modeling_llama.repeat_kv(kt, rep), modeling_llama.repeat_kv(vt, rep)) if rep > 1 else (kt, vt)
         out = F.scaled_dot_product_attention(qt, kr, vr, attn_mask=attention_mask, dropout_p=0.0,

@@ -222,3 +222,24 @@ def test_prefix_s_forward_under_either_mask(patched, kind):
             with pytest.raises(ValueError, match="padding"):
                 model(input_ids=ids, attention_mask=mask, past_key_values=cache)
             assert cache.layers[0].prefix_k is None
+
+
+@pytest.mark.parametrize("padded", [False, True])
+def test_padded_prefix_needs_a_prefix_mask(patched, padded):
+    """Tokens that were hidden in the prefix's forward would be seen by every step after it."""
+    model, ids = cpu_model(), torch.randint(0, 50, (1, 20))
+    mask = torch.ones(1, 20, dtype=torch.long)
+    if padded:
+        mask[0, :3] = 0
+    with torch.no_grad():
+        cache = patched.build_shared_prefix_cache(model, page_size=16)
+        model(input_ids=ids, attention_mask=mask, past_key_values=cache)
+        if padded:
+            with pytest.raises(ValueError, match="prefix_mask"):
+                cache.begin(2, 64)
+            assert cache.n_seq == 0
+            cache.begin(2, 64, prefix_mask=mask[0].bool())
+            assert cache.prefix_mask.tolist() == mask[0].tolist()
+        else:
+            cache.begin(2, 64)
+        assert cache.n_seq == 2

@@ -188,8 +188,12 @@ class SharedPrefixCache(Cache):
         uniform = min(new) == tokens
         add = torch.full((self.n_seq,), tokens, dtype=torch.int32, device=dev) if uniform else \
             torch.tensor(new, dtype=torch.int32, device=dev)
+        # committed in place; the status is the cache's own, which keeps the bits of every step, replayed ones too
+        i32, i64 = dict(dtype=torch.int32, device=dev), dict(dtype=torch.int64, device=dev)
         p = self.plan = plan_pages(self.lens, add, self.block_table, self.free_pages, self.n_free, self.page_size, n,
-                                   base_pos=self.prefix_len)
+                                   base_pos=self.prefix_len,
+                                   out=PagePlan(torch.empty(self.n_seq + 1, **i32), torch.empty(n, **i64), torch.empty(n, **i32),
+                                                torch.empty(n, **i64), self.lens, self.n_free, self.status))
         # packed row t comes from row seq * tokens + its place in the sequence; row n stands for none
         self._rows = None
         if not uniform:
@@ -207,8 +211,10 @@ class SharedPrefixCache(Cache):
             q, k, v = q.index_select(0, at), k.index_select(0, at), v.index_select(0, at)
         q = append_pages(q, k, v, p.slots, p.positions, layer.k_pages, layer.v_pages, inv_freq=self.inv_freq,
                          rope_scaling=self.rope_scaling, status=self.status)
+        # a step that the plan refuses on the device has no tokens: its rows stay 0 (ragged steps: `back` below)
+        out = q.new_zeros(q.shape) if rows is None else None
         out = shared_prefix_attention(q, layer.prefix_k, layer.prefix_v, layer.k_pages, layer.v_pages, self.block_table,
-                                      p.lens, p.cu_new, scaling, prefix_mask=self.prefix_mask, status=self.status)
+                                      p.lens, p.cu_new, scaling, prefix_mask=self.prefix_mask, out=out, status=self.status)
         if rows is None:
             return out
         back = torch.zeros((n + 1,) + out.shape[1:], dtype=out.dtype, device=out.device)
@@ -226,10 +232,10 @@ class SharedPrefixCache(Cache):
         self.host_lens = keep
 
     def device_status(self) -> int:
-        """OR of the HC_DEV_* bits of the steps so far (synchronises)."""
-        if self.n_seq == 0:
-            return 0
-        return int(self.status) | (int(self.plan.status) if self.plan is not None else 0)
+        """OR of the HC_DEV_* bits of the steps since begin(), replays included (synchronises). HC_DEV_CAPACITY: a step
+        did not fit the pages and left everything as it was, with outputs of 0. HC_DEV_TIMEOUT: a step's outputs are
+        worthless."""
+        return 0 if self.n_seq == 0 else int(self.status)
 
     # ------------------------------------------------------------------ what transformers may ask of a cache
     # Its own versions work on dense keys and values of a layer, here the prefix of all sequences.

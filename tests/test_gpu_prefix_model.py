@@ -272,3 +272,47 @@ def test_rotary_that_follows_the_length(kind):
         finally:
             hc.uninstall_monkeypatch()
     assert (got - ref).abs().max() <= TOL[torch.float32] * ref.abs().max()
+
+
+def test_replays_past_the_pages_are_reported():
+    """A captured step replayed until the pages are full: the refused replays leave the tables alone and outputs of 0, and
+    their bit outlasts the steps behind them."""
+    import hotcold_kv_cache_b200 as hc
+    from hotcold_kv_cache_b200 import _lib
+    g = torch.Generator(device="cuda").manual_seed(1)
+    rnd = lambda *s: torch.randn(s, generator=g, device="cuda", dtype=torch.float32).half()  # noqa: E731
+    cache = hc.SharedPrefixCache(1, torch.ones(32), page_size=16)
+    cache.set_prefix(0, rnd(2, 50, 64), rnd(2, 50, 64))
+    cache.begin(3, 32)
+    q, k, v = rnd(3, 8, 64), rnd(3, 2, 64), rnd(3, 2, 64)
+
+    def step():
+        cache.start_step(3, 1)
+        return cache.attend(0, q, k, v, 0.125)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for _ in range(31):
+        graph.replay()
+        assert bool((out != 0).any(-1).all())
+    assert cache.lens.tolist() == [32] * 3 and cache.device_status() == 0
+    pages = cache.layers[0].k_pages.clone()
+    for _ in range(2):
+        graph.replay()
+    assert not out.any() and cache.lens.tolist() == [32] * 3 and int(cache.n_free) == 0
+    assert torch.equal(cache.layers[0].k_pages, pages)
+    cache.refresh_lens()
+    cache.release([3, 0, 32])
+    with pytest.raises(RuntimeError):
+        step()  # the third sequence is full
+    cache.release([3, 0, 31])
+    assert bool((step() != 0).any(-1).all()) and cache.lens.tolist() == [4, 1, 32]
+    assert cache.device_status() == _lib.HC_DEV_CAPACITY
+    cache.begin(3, 32)
+    assert cache.device_status() == 0

@@ -120,7 +120,13 @@ class SharedPrefixCache(Cache):
             raise ValueError("the prefix's attention mask hid some of its tokens: begin(prefix_mask=) says which stay hidden")
         if n_seq < 1 or max_new_tokens < 1:
             raise ValueError("begin() needs at least one sequence and one new token")
-        dev, (Hk, _, D) = first.prefix_k.device, first.prefix_k.shape
+        dev, (Hk, P, D) = first.prefix_k.device, first.prefix_k.shape
+        if prefix_mask is not None:
+            if prefix_mask.dtype.is_floating_point:
+                raise TypeError(f"prefix_mask must be bool or whole numbers (0 leaves a token out), not {prefix_mask.dtype}")
+            if prefix_mask.numel() != P:
+                raise ValueError(f"prefix_mask has {prefix_mask.numel()} values for a prefix of {P} tokens")
+            prefix_mask = (prefix_mask.reshape(P) != 0).to(device=dev, dtype=torch.uint8)
         ps = self.page_size
         self.n_seq, self.max_blocks = int(n_seq), -(-int(max_new_tokens) // ps)
         most = self.n_seq * self.max_blocks
@@ -131,7 +137,7 @@ class SharedPrefixCache(Cache):
         self.free_pages = torch.arange(self.n_pages, **z)
         self.n_free = torch.full((1,), self.n_pages, **z)
         self.status = torch.zeros(1, **z)
-        self.prefix_mask = None if prefix_mask is None else prefix_mask.to(device=dev, dtype=torch.uint8).contiguous()
+        self.prefix_mask = prefix_mask
         self._read_rotary(dev)
         for layer in self.layers:
             if layer.prefix_k is None:

@@ -243,3 +243,16 @@ def test_padded_prefix_needs_a_prefix_mask(patched, padded):
         else:
             cache.begin(2, 64)
         assert cache.n_seq == 2
+
+
+def test_prefix_mask_is_checked_before_any_step():
+    cache, _ = cpu_cache()
+    for bad in (torch.ones(5, dtype=torch.bool), torch.ones(2, 8, dtype=torch.bool), torch.ones(0, dtype=torch.uint8)):
+        with pytest.raises(ValueError, match="prefix of 8 tokens"):
+            cache.begin(2, 16, prefix_mask=bad)
+    with pytest.raises(TypeError, match="prefix_mask"):  # an additive mask's 0 means the opposite
+        cache.begin(2, 16, prefix_mask=torch.zeros(8))
+    assert cache.n_seq == 0
+    for mask in (torch.tensor([1, 0, 256, 1, 1, 1, 1, 1]), torch.tensor([[True, False] + [True] * 6])):
+        cache.begin(2, 16, prefix_mask=mask)
+        assert cache.prefix_mask.dtype is torch.uint8 and cache.prefix_mask.tolist() == [1, 0, 1, 1, 1, 1, 1, 1]

@@ -24,6 +24,19 @@ from transformers.cache_utils import Cache, CacheLayerMixin
 from .prefix import PagePlan, append_pages, plan_pages, release_pages, shared_prefix_attention
 
 
+# What the kernels take (include/hotcold_b200.h); checked here before a step moves lengths and pages.
+MAX_SEQ, MAX_ROWS, MAX_PREFIX, MAX_OWN, MAX_POOL_ROWS = 4096, 65536, 1 << 24, 1 << 30, (1 << 31) - 1
+
+
+def check_heads(Hq: int, Hk: int, D: int, dtype):
+    if D not in (64, 128):
+        raise ValueError(f"a shared-prefix cache takes a head_dim of 64 or 128, not {D}")
+    if Hq not in (Hk, 2 * Hk, 4 * Hk, 8 * Hk):
+        raise ValueError(f"a shared-prefix cache takes 1, 2, 4 or 8 query heads a key head, not {Hq} over {Hk}")
+    if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+        raise TypeError(f"a shared-prefix cache takes float32, float16 or bfloat16, not {dtype}")
+
+
 class SharedPrefixLayer(CacheLayerMixin):
     """One layer: the prefix's post-RoPE keys and values (Hk, P, D) and the pages of the sequences' own."""
     is_compileable = False
@@ -121,16 +134,31 @@ class SharedPrefixCache(Cache):
         if n_seq < 1 or max_new_tokens < 1:
             raise ValueError("begin() needs at least one sequence and one new token")
         dev, (Hk, P, D) = first.prefix_k.device, first.prefix_k.shape
+        for layer in self.layers:
+            if layer.prefix_k is None:
+                raise RuntimeError("begin() comes after the prefix's forward")
+            if any(x.shape != first.prefix_k.shape or x.dtype is not first.prefix_k.dtype or x.device != dev
+                   for x in (layer.prefix_k, layer.prefix_v)):
+                raise ValueError("the prefix's keys and values must share shape, dtype and device over all layers")
+        check_heads(Hk, Hk, D, first.prefix_k.dtype)
+        ps = self.page_size
+        max_blocks = -(-int(max_new_tokens) // ps)
+        most = int(n_seq) * max_blocks
+        n_pages = most if pool_tokens is None else max(1, min(most, -(-int(pool_tokens) // ps)))
+        if n_seq > MAX_SEQ or P > MAX_PREFIX or max_blocks * ps > MAX_OWN or n_pages * Hk * ps > MAX_POOL_ROWS:
+            raise ValueError(f"a shared-prefix cache takes up to {MAX_SEQ} sequences, a prefix of {MAX_PREFIX} tokens, {MAX_OWN} "
+                             f"own tokens a sequence and 2^31 - 1 rows of a head a pool; asked for {n_seq}, {P}, "
+                             f"{max_blocks * ps} and {n_pages * Hk * ps}")
+        freq = self.inv_freq if self.rotary is None else self.rotary.inv_freq
+        if freq.numel() * 2 != D:
+            raise ValueError(f"{freq.numel()} rotary frequencies do not turn a whole head of {D}")
         if prefix_mask is not None:
             if prefix_mask.dtype.is_floating_point:
                 raise TypeError(f"prefix_mask must be bool or whole numbers (0 leaves a token out), not {prefix_mask.dtype}")
             if prefix_mask.numel() != P:
                 raise ValueError(f"prefix_mask has {prefix_mask.numel()} values for a prefix of {P} tokens")
             prefix_mask = (prefix_mask.reshape(P) != 0).to(device=dev, dtype=torch.uint8)
-        ps = self.page_size
-        self.n_seq, self.max_blocks = int(n_seq), -(-int(max_new_tokens) // ps)
-        most = self.n_seq * self.max_blocks
-        self.n_pages = most if pool_tokens is None else max(1, min(most, -(-int(pool_tokens) // ps)))
+        self.n_seq, self.max_blocks, self.n_pages = int(n_seq), max_blocks, n_pages
         z = dict(dtype=torch.int32, device=dev)
         self.lens = torch.zeros(self.n_seq, **z)
         self.block_table = torch.full((self.n_seq, self.max_blocks), -1, **z)
@@ -140,8 +168,6 @@ class SharedPrefixCache(Cache):
         self.prefix_mask = prefix_mask
         self._read_rotary(dev)
         for layer in self.layers:
-            if layer.prefix_k is None:
-                raise RuntimeError("begin() comes after the prefix's forward")
             layer.k_pages = torch.empty((self.n_pages, Hk, ps, D), dtype=layer.prefix_k.dtype, device=dev)
             layer.v_pages = torch.empty_like(layer.k_pages)
         self.host_lens = [0] * self.n_seq
@@ -181,6 +207,8 @@ class SharedPrefixCache(Cache):
         self._begun("a step")
         if batch != self.n_seq:
             raise ValueError(f"the batch has {batch} rows, the cache {self.n_seq} sequences")
+        if batch * tokens > MAX_ROWS:
+            raise ValueError(f"a step takes up to {MAX_ROWS} rows, padding included, not {batch} x {tokens}: send it in parts")
         new = self._next if self._next is not None else [tokens] * self.n_seq
         if max(new) > tokens:
             raise ValueError(f"next_lens names {max(new)} tokens of a row of {tokens}")
@@ -299,6 +327,7 @@ def shared_prefix_forward(attn, hidden_states, position_embeddings, attention_ma
     k = attn.k_proj(hidden_states).view(b, t, -1, d)
     v = attn.v_proj(hidden_states).view(b, t, -1, d)
     if cache.n_seq == 0:
+        check_heads(q.shape[2], k.shape[2], d, k.dtype)
         if b != 1:
             raise ValueError("the prefix goes through the model as one sequence; begin() then opens the batch")
         qt, kt, vt = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
@@ -321,6 +350,9 @@ def shared_prefix_forward(attn, hidden_states, position_embeddings, attention_ma
         if t > 1 and cache._next is None and hides_keys(attention_mask):
             raise ValueError("the attention mask hides keys of a step: name its padding with next_lens(), and the prefix's "
                              "with begin(prefix_mask=); a shared-prefix cache does not read the mask")
+        pre = cache.layers[0].prefix_k
+        if k.dtype is not pre.dtype or k.device != pre.device:
+            raise ValueError(f"a step of {k.dtype} on {k.device} behind a prefix of {pre.dtype} on {pre.device}")
         cache.start_step(b, t)
     out = cache.attend(li, q.reshape(b * t, -1, d), k.reshape(b * t, -1, d), v.reshape(b * t, -1, d), float(attn.scaling))
     return attn.o_proj(out.reshape(b, t, -1)), None

@@ -256,3 +256,56 @@ def test_prefix_mask_is_checked_before_any_step():
     for mask in (torch.tensor([1, 0, 256, 1, 1, 1, 1, 1]), torch.tensor([[True, False] + [True] * 6])):
         cache.begin(2, 16, prefix_mask=mask)
         assert cache.prefix_mask.dtype is torch.uint8 and cache.prefix_mask.tolist() == [1, 0, 1, 1, 1, 1, 1, 1]
+
+
+def test_limits_are_checked_before_a_step_moves_anything():
+    """What the kernels refuse is refused before lengths and pages move: rows with padding, sequences, pools, heads."""
+    from hotcold_kv_cache_b200.prefix_cache import SharedPrefixCache
+    cache, _ = cpu_cache()
+    cache.begin(256, 512)
+    cache.next_lens([300] + [1] * 255)
+    with pytest.raises(ValueError, match="65536"):
+        cache.start_step(256, 300)
+    assert cache.host_lens == [0] * 256 and not cache.lens.any() and int(cache.n_free) == cache.n_pages
+    assert (cache.block_table == -1).all() and cache.plan is None
+    cache, _ = cpu_cache()
+    for n_seq, new in ((4097, 16), (2, (1 << 30) + 1), (4096, 1 << 20)):
+        with pytest.raises(ValueError, match="up to"):
+            cache.begin(n_seq, new)
+        assert cache.n_seq == 0 and cache.layers[0].k_pages is None
+    cache.begin(4096, 16, pool_tokens=64)
+    for D, dtype, freq, err in ((96, torch.float32, 48, ValueError), (64, torch.float64, 32, TypeError),
+                                (64, torch.float32, 16, ValueError)):
+        cache, k = SharedPrefixCache(1, torch.ones(freq)), torch.zeros(2, 8, D, dtype=dtype)
+        cache.set_prefix(0, k, k)
+        with pytest.raises(err):
+            cache.begin(2, 16)
+        assert cache.n_seq == 0
+    cache = SharedPrefixCache(2, torch.ones(32))
+    cache.set_prefix(0, torch.zeros(2, 8, 64), torch.zeros(2, 8, 64))
+    with pytest.raises(RuntimeError, match="begin"):  # the second layer has none
+        cache.begin(2, 16)
+    cache.set_prefix(1, torch.zeros(2, 9, 64), torch.zeros(2, 9, 64))
+    with pytest.raises(ValueError, match="all layers"):
+        cache.begin(2, 16)
+    assert cache.n_seq == 0
+
+
+def test_model_s_heads_and_types_are_checked(patched):
+    """A group of 3 query heads is refused in the prefix's forward, a step of another type before it moves anything."""
+    from transformers import LlamaConfig, LlamaForCausalLM
+    ids = torch.randint(0, 50, (1, 20))
+    with torch.no_grad():
+        odd = LlamaForCausalLM(LlamaConfig(vocab_size=50, hidden_size=192, intermediate_size=64, num_hidden_layers=1,
+                                           num_attention_heads=3, num_key_value_heads=1, head_dim=64)).eval()
+        cache = patched.build_shared_prefix_cache(odd, page_size=16)
+        with pytest.raises(ValueError, match="query heads"):
+            odd(input_ids=ids, past_key_values=cache)
+        assert cache.layers[0].prefix_k is None
+        model = cpu_model()
+        cache = patched.build_shared_prefix_cache(model, page_size=16)
+        model(input_ids=ids, past_key_values=cache)
+        cache.begin(1, 64)
+        with pytest.raises(ValueError, match="behind a prefix"):
+            model.to(torch.bfloat16)(input_ids=ids, past_key_values=cache)
+        assert cache.host_lens == [0] and cache.plan is None

@@ -35,7 +35,12 @@ namespace hc {
 
 constexpr int kMmaThreads = 384, kMmaR = 256, kMmaK = 128;
 constexpr int kPieces = 8;    // pieces listed ahead
-constexpr float kLazy = 8.f;  // log2 of how far P may exceed 1 before O is rescaled
+
+template <int DT>
+struct PRange {
+  static constexpr float kLift = DT == HC_F16 ? 11.f : 0.f;  // log2 of what P of a row's maximum is
+  static constexpr float kLazy = DT == HC_F16 ? 4.f : 8.f;   // log2 of how far P may exceed that before O is rescaled
+};
 
 template <int D>
 struct MmaSmem {
@@ -407,7 +412,7 @@ __device__ __forceinline__ void rows_tiles(const Soft& f, uint32_t& nt, float& m
         }
       }
       const float mt = fmaxf(mx0, mx1) * f.sc;
-      if (__any_sync(0xffffffffu, f.r < f.t.nr && mt > m + kLazy)) {  // rows of no token hold anything: no vote
+      if (__any_sync(0xffffffffu, f.r < f.t.nr && mt > m + PRange<DT>::kLazy)) {  // rows of no token hold anything: no vote
         const float mn = fmaxf(m, mt), al = ex2_approx(m - (mn == kNegInf ? 0.f : mn));
         m = mn;
         l *= al;
@@ -423,7 +428,7 @@ __device__ __forceinline__ void rows_tiles(const Soft& f, uint32_t& nt, float& m
           }
         }
       }
-      const float ref = m == kNegInf ? 0.f : m;
+      const float ref = m == kNegInf ? 0.f : m - PRange<DT>::kLift;
       float l0 = 0.f, l1 = 0.f;
 #pragma unroll 1
       for (int j = 0; j < 4; ++j) {
@@ -477,7 +482,7 @@ __device__ __forceinline__ void rows_out(const Soft& f, float m, float l, bool a
       }
     }
   }
-  if (f.r < nr) ml[blk + f.r] = make_float2(m, l);
+  if (f.r < nr) ml[blk + f.r] = make_float2(m - PRange<DT>::kLift, l);
 }
 
 // A thread per key: the key tiles of a piece of up to N rows, and its maxima and sums.
@@ -530,7 +535,7 @@ __device__ __forceinline__ bool cols_tiles(const Soft& f, uint32_t& nt, float2* 
       wait_bar(f.pv_done, (nt - 1) & 1, f.dead, f.a.status);
       tc_fence_after();
     }
-    const bool up = (lane < nr && t0 > m0 + kLazy) || (N > 32 && 32 + lane < nr && t1 > m1 + kLazy);
+    const bool up = (lane < nr && t0 > m0 + PRange<DT>::kLazy) || (N > 32 && 32 + lane < nr && t1 > m1 + PRange<DT>::kLazy);
     if (__any_sync(0xffffffffu, up)) {
       const float n0 = fmaxf(m0, t0), n1 = fmaxf(m1, t1);
       const float a0 = ex2_approx(m0 - (n0 == kNegInf ? 0.f : n0)), a1 = ex2_approx(m1 - (n1 == kNegInf ? 0.f : n1));
@@ -550,7 +555,7 @@ __device__ __forceinline__ bool cols_tiles(const Soft& f, uint32_t& nt, float2* 
         tmem_wait_st();
       }
     }
-    const float r0 = m0 == kNegInf ? 0.f : m0, r1 = m1 == kNegInf ? 0.f : m1;
+    const float r0 = m0 == kNegInf ? 0.f : m0 - PRange<DT>::kLift, r1 = m1 == kNegInf ? 0.f : m1 - PRange<DT>::kLift;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
       const float pr = ex2_approx(fmaf(s[n], f.sc, -__shfl_sync(0xffffffffu, n < 32 ? r0 : r1, n & 31)));
@@ -575,7 +580,7 @@ __device__ __forceinline__ bool cols_tiles(const Soft& f, uint32_t& nt, float2* 
   if (N > 32) red[f.warp4 * 64 + 32 + lane] = w1;
   named_sync(1 + f.x, 128);
   if (f.r < nr)
-    ml[p.row0 + f.r] = make_float2(f.r < 32 ? m0 : m1, red[f.r] + red[64 + f.r] + red[128 + f.r] + red[192 + f.r]);
+    ml[p.row0 + f.r] = make_float2((f.r < 32 ? m0 : m1) - PRange<DT>::kLift, red[f.r] + red[64 + f.r] + red[128 + f.r] + red[192 + f.r]);
   return any;
 }
 

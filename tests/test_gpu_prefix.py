@@ -400,6 +400,37 @@ def test_sharp_scores(scale):
     check(s, "f16", got, lse, 10)
 
 
+@pytest.mark.parametrize("dt", ["f16", "bf16", "f32"])
+@pytest.mark.parametrize("Hq,Hk,D,T", [(8, 2, 128, 1), (8, 2, 128, 10), (16, 2, 64, 13), (32, 4, 64, 608)])
+def test_sink_before_a_long_prefix(dt, Hq, Hk, D, T):
+    """One key of a probability near 1 and 100 thousand others near 2^-26 each, which together are 0.15 % of the weight and
+    all of the result, since the first key's value is 0."""
+    import hotcold_kv_cache_b200 as hc
+    P = 100000
+    s = state(14, dt, Hq, Hk, D, P, 16, [0], [T], layout="heads")
+    s["q"].zero_()
+    s["q"][..., 0] = 1
+    s["scaling"] = math.log(2)  # a score is 2's exponent
+    s["prefix_k"][..., 0] = (-26 + 0.125 * s["prefix_k"][..., 0].float()).to(DT[dt])
+    s["k_pages"][..., 0] = -26
+    for v in (s["prefix_v"], s["v_pages"]):
+        v.copy_((1 + 0.25 * v.float()).to(DT[dt]))
+    s["prefix_k"][:, 0, 0] = 0
+    s["prefix_v"][:, 0] = 0
+    got, lse = hc.shared_prefix_attention(**s, return_lse=True)
+    ref, rl, A, S = R.attend(s["q"], s["prefix_k"], s["prefix_v"], s["k_pages"], s["v_pages"], s["block_table"], s["lens"],
+                             s["cu_new"], s["scaling"])
+    assert 1e-3 < float(ref.mean()) < 2e-3
+    # f16 holds a probability 2^11 times larger; what is below its normal numbers is off by up to 2^-25, and each of the
+    # P + T probabilities so by 2^-36 of the largest
+    lost = (P + T) * 2.0 ** -36 * float(s["prefix_v"].abs().max()) if dt == "f16" else 0.0
+    tol = R.attend_tolerance(DT[dt], D, P + T, ref, A, S) + lost
+    worst = ((got.double() - ref).abs() / tol).max()
+    assert worst <= 1, f"off by {float(worst):.2f} of the tolerance"
+    assert ((lse.double() - rl).abs() <= D * 2.0 ** -22 * S + 2.0 ** -20 + 2.0 ** -22 * rl.abs() +
+            8 * math.sqrt(P + T) * 2.0 ** -24).all()
+
+
 @pytest.mark.parametrize("dt", ["f16", "f32"])
 def test_another_stream_and_a_captured_graph(dt):
     import hotcold_kv_cache_b200 as hc

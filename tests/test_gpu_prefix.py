@@ -431,6 +431,60 @@ def test_sink_before_a_long_prefix(dt, Hq, Hk, D, T):
             8 * math.sqrt(P + T) * 2.0 ** -24).all()
 
 
+def relaid(x, how, fill=math.nan):
+    """x (heads, tokens, D) with the same values in another layout, the memory around it not finite."""
+    H, N, D = x.shape
+    if how == "slice":  # tokens in the middle of a longer buffer, between heads of another use
+        big = torch.full((H + 2, N + 24, D), fill, dtype=x.dtype, device=x.device)
+        view = big[1:H + 1, 16:16 + N]
+    elif how == "fused":  # heads of a fused projection's rows
+        big = torch.full((N, H + 3, D), fill, dtype=x.dtype, device=x.device)
+        view = big[:, 2:2 + H].transpose(0, 1)
+    elif how == "wide":  # rows of D inside longer ones
+        big = torch.full((H, N, D + 32), fill, dtype=x.dtype, device=x.device)
+        view = big[..., 16:16 + D]
+    view.copy_(x)
+    return view
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("lay_q,lay_k,lay_v", [("fused", "slice", "slice"), ("slice", "fused", "slice"), ("wide", "wide", "fused"),
+                                               ("fused", "slice", "fused")])
+@pytest.mark.parametrize("case", [3, 5, 13, 14])
+def test_attention_reads_strided_inputs_in_place(dt, lay_q, lay_k, lay_v, case):
+    """Queries as slices of a fused projection, prefixes as slices of longer buffers, keys and values laid out differently:
+    the bits of the contiguous call."""
+    import hotcold_kv_cache_b200 as hc
+    Hq, Hk, D, P, ps, ctx, new = CASES[case]
+    s = state(200 + case, dt, Hq, Hk, D, P, ps, ctx, new, mask=0.8 if case == 3 else None, layout="heads")
+    want, lse = hc.shared_prefix_attention(**s, return_lse=True)
+    check(s, dt, want, lse, int(np.sum(new)))
+    t = dict(s, q=relaid(s["q"].transpose(0, 1), lay_q).transpose(0, 1), prefix_k=relaid(s["prefix_k"], lay_k),
+             prefix_v=relaid(s["prefix_v"], lay_v))
+    assert not t["q"].is_contiguous() and not t["prefix_k"].is_contiguous()
+    assert torch.equal(hc.shared_prefix_attention(**t), want)
+
+
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+@pytest.mark.parametrize("T", [1, 5])
+@pytest.mark.parametrize("Hk,P", [(1, 1), (1, 2), (1, 300), (4, 1)])
+def test_strides_of_single_heads_and_tokens_say_nothing(dt, T, Hk, P):
+    import hotcold_kv_cache_b200 as hc
+    D = 128
+    s = state(15, dt, 2 * Hk, Hk, D, P, 16, [20], [T], layout="heads")
+    want, lse = hc.shared_prefix_attention(**s, return_lse=True)
+    check(s, dt, want, lse, T)
+    t = dict(s)
+    for name, x in (("prefix_k", s["prefix_k"]), ("prefix_v", s["prefix_v"])):
+        t[name] = x.as_strided(x.shape, (3 if Hk == 1 else x.stride(0), 5 if P == 1 else x.stride(1), 1))
+    if T == 1:
+        t["q"] = s["q"].as_strided(s["q"].shape, (7, D, 1))
+    assert torch.equal(hc.shared_prefix_attention(**t), want)
+    odd = torch.zeros(T, 2 * Hk, D + 1, dtype=DT[dt], device="cuda")[..., 1:]  # rows that do not start on 16 bytes: copied
+    odd.copy_(s["q"])
+    assert torch.equal(hc.shared_prefix_attention(**dict(s, q=odd)), want)
+
+
 @pytest.mark.parametrize("dt", ["f16", "f32"])
 def test_another_stream_and_a_captured_graph(dt):
     import hotcold_kv_cache_b200 as hc

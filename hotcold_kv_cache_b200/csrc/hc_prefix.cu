@@ -261,9 +261,10 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(PrefixArgs 
   __syncthreads();
   for (int b = tid; b < s.n_seq; b += kMergeThreads)
     if (a.cu_new[b] <= t && t < a.cu_new[b + 1]) s_b = b;
-  if (t >= R) return;  // rows behind the last sequence are left as they were
+  if (t >= R) return;  // rows behind the last sequence are left as they were ...
   const LineGeom g(s, R);
   __syncthreads();
+  if (s_b < 0) return;  // ... and so are rows before the first
   // the blocks of partial rows over these rows, in a fixed order: segment j < nch the prefix chunk j, segment
   // nch the own pages; where a CTA ran two streams over the keys, both of its blocks
   if (warp == 0) {
@@ -277,7 +278,7 @@ __global__ void __launch_bounds__(kMergeThreads) prefix_merge_kernel(PrefixArgs 
       rows = min(g.tt, R - tok0) * s.G, q0 = (t - tok0) * s.G;
       lo = line_div(v0, W), hi = line_div(v0 + (int64_t)(tiles - 1) * g.pre.a, W);
       row = s.dup * (((int64_t)h * s.nch + lane) * s.T + tok0) * s.G;
-    } else if (lane == s.nch && s_b >= 0) {
+    } else if (lane == s.nch) {
       const SeqLens q = seq_lens(a, s_b);
       const int r = (t - q.cu) / g.tt, nr = ceil_div(q.n, g.tt), tok1 = min(q.n, (r + 1) * g.tt);
       const int tiles = ceil_div(seq_keys(q, tok1), s.kt);

@@ -228,7 +228,7 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k_pages, v_pages, block_table
     sequence b's n_b attends the prefix keys where prefix_mask (P) bool or uint8 is set (None: all) and
     its own keys j <= lens[b] - n_b + i. Returns out (T,Hq,D), contiguous, and with return_lse the
     natural-log sum of exponentials (T,Hq) float32 too. A row that attends nothing is 0 (lse -inf); rows
-    from cu_new[n_seq] on are left as they were. A table entry outside the pool reads as zero keys and
+    of no sequence (before cu_new[0], from cu_new[n_seq] on) are left as they were. A table entry outside the pool reads as zero keys and
     values and sets HC_DEV_INDEX in status (1) int32, when given."""
     dev = _cuda("q", q)
     if q.dim() != 3:

@@ -424,8 +424,8 @@ HC_API int hc_append_pages(const void* q, int64_t q_st, int64_t q_sh, const void
  * prefix_mask[j] != 0 (mask NULL: all) and own key j <= lens[b] - n_b + i (lens counts the step's
  * tokens). Prefix keys and values are (Hk,P,D) with strides over heads and tokens. The prefix is read
  * once for the whole batch. out (T,Hq,D) contiguous; lse (T,Hq) fp32, or NULL: the natural log of the
- * sum of exponentials. A row that attends nothing is 0 with lse -inf; rows from cu_new[n_seq] on are
- * left as they were. A block table entry outside the pool reads as zero keys and values, a length
+ * sum of exponentials. A row that attends nothing is 0 with lse -inf; rows of no sequence
+ * (before cu_new[0], from cu_new[n_seq] on) are left as they were. A block table entry outside the pool reads as zero keys and values, a length
  * outside max_blocks pages is cut, and both set HC_DEV_INDEX; a wait inside the kernel that ran out
  * sets HC_DEV_TIMEOUT, and the call's results are then worthless. T <= 65536. Scratch from
  * hc_shared_prefix_attention_scratch_bytes (asked for with the call's device current: the work is

@@ -485,6 +485,24 @@ def test_strides_of_single_heads_and_tokens_say_nothing(dt, T, Hk, P):
     assert torch.equal(hc.shared_prefix_attention(**dict(s, q=odd)), want)
 
 
+@pytest.mark.parametrize("dt", ["f32", "f16"])
+def test_rows_of_no_sequence_are_left_alone(dt):
+    """The sequences' rows may start behind the first and end before the last."""
+    import hotcold_kv_cache_b200 as hc
+    s = state(16, dt, 8, 2, 128, 200, 16, [30, 0, 9], [1, 5, 40], pad=3)
+    want, lse = hc.shared_prefix_attention(**s, return_lse=True)
+    check(s, dt, want, lse, 46)
+    s["q"] = torch.cat([torch.full_like(s["q"][:7], math.nan), s["q"]])
+    s["cu_new"] = s["cu_new"] + 7
+    out = torch.full_like(s["q"], 7.0)
+    hc.shared_prefix_attention(**s, out=out)
+    lo, hi = out[:7], out[53:]
+    assert (lo == 7.0).all() and (hi == 7.0).all()
+    # row tiles fall elsewhere: sums in another order
+    shifted = dict(s, q=s["q"][7:], cu_new=s["cu_new"] - 7)
+    check(shifted, dt, out[7:], lse, 46)
+
+
 @pytest.mark.parametrize("dt", ["f16", "f32"])
 def test_another_stream_and_a_captured_graph(dt):
     import hotcold_kv_cache_b200 as hc

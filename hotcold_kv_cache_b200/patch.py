@@ -86,7 +86,8 @@ def install_monkeypatch(enable_debug: bool = True):
                         attention_mask: Optional[torch.Tensor] = None, past_key_values: Optional[Cache] = None,
                         cache_position: Optional[torch.LongTensor] = None, **kwargs):
         if isinstance(past_key_values, SharedPrefixCache):
-            return shared_prefix_forward(self, hidden_states, position_embeddings, attention_mask, past_key_values)
+            return shared_prefix_forward(self, hidden_states, position_embeddings, attention_mask, past_key_values,
+                                         kwargs.get("position_ids"))
         kvctrl = ACTIVE_KVCTRL
         if kvctrl is None:
             return _ORIG(self, hidden_states=hidden_states, position_embeddings=position_embeddings,

@@ -315,11 +315,19 @@ def hides_keys(mask) -> bool:
     return not bool((last if mask.dtype is torch.bool else last == 0).all())
 
 
-def shared_prefix_forward(attn, hidden_states, position_embeddings, attention_mask, cache: SharedPrefixCache):
+def moved(position_ids: Optional[torch.Tensor], tokens: int) -> bool:
+    """Whether a forward's positions are others than 0 to tokens - 1. Synchronises; under capture it says no."""
+    if position_ids is None or (position_ids.is_cuda and torch.cuda.is_current_stream_capturing()):
+        return False
+    return not torch.equal(position_ids.reshape(-1), torch.arange(tokens, dtype=position_ids.dtype, device=position_ids.device))
+
+
+def shared_prefix_forward(attn, hidden_states, position_embeddings, attention_mask, cache: SharedPrefixCache,
+                          position_ids: Optional[torch.Tensor] = None):
     """LlamaAttention.forward over a SharedPrefixCache: before begin() the prefix's forward (transformers' RoPE and
-    stock causal attention, as the patched prompt forward), after it the batch's step, whose positions and mask
-    are the cache's own: padding comes from next_lens(). A mask that hides keys from a step of several tokens is
-    refused where next_lens() says nothing."""
+    stock causal attention, as the patched prompt forward; at positions 0 to P - 1, since own tokens go on from P),
+    after it the batch's step, whose positions and mask are the cache's own: padding comes from next_lens(). A mask
+    that hides keys from a step of several tokens is refused where next_lens() says nothing."""
     from transformers.models.llama import modeling_llama
     b, t, _ = hidden_states.shape
     li, d = int(attn.layer_idx), int(attn.head_dim)
@@ -330,6 +338,8 @@ def shared_prefix_forward(attn, hidden_states, position_embeddings, attention_ma
         check_heads(q.shape[2], k.shape[2], d, k.dtype)
         if b != 1:
             raise ValueError("the prefix goes through the model as one sequence; begin() then opens the batch")
+        if li == 0 and cache.layers[0].prefix_k is None and moved(position_ids, t):
+            raise ValueError("the prefix sits at positions 0 to P - 1: own tokens go on from P")
         qt, kt, vt = q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2)
         cos, sin = position_embeddings
         if attention_mask is not None and not (isinstance(attention_mask, torch.Tensor) and attention_mask.dim() == 4):

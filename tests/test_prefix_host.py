@@ -309,3 +309,20 @@ def test_model_s_heads_and_types_are_checked(patched):
         with pytest.raises(ValueError, match="behind a prefix"):
             model.to(torch.bfloat16)(input_ids=ids, past_key_values=cache)
         assert cache.host_lens == [0] and cache.plan is None
+
+
+def test_prefix_sits_at_the_first_positions(patched):
+    """Own tokens go on from the prefix's length, so a prefix at other positions is refused."""
+    model, ids = cpu_model(), torch.randint(0, 50, (1, 20))
+    at = torch.arange(20)[None]
+    padded = (torch.tensor([[0] * 3 + [1] * 17]).cumsum(1) - 1).clamp(min=0)  # as for three tokens of padding on the left
+    with torch.no_grad():
+        for bad in (at + 5, padded):
+            cache = patched.build_shared_prefix_cache(model, page_size=16)
+            with pytest.raises(ValueError, match="positions 0 to"):
+                model(input_ids=ids, position_ids=bad, past_key_values=cache)
+            assert cache.layers[0].prefix_k is None
+        for good in (at, at.int(), None):
+            cache = patched.build_shared_prefix_cache(model, page_size=16)
+            model(input_ids=ids, position_ids=good, past_key_values=cache)
+            assert cache.prefix_len == 20

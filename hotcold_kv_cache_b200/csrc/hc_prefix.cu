@@ -4,7 +4,10 @@
 //
 // 16-bit types run on the tensor cores (hc_prefix_mma.cu). prefix_simt_kernel serves fp32 layers: 64 rows x
 // 64 keys with fp32 FMAs; scores and probabilities pass through shared memory, the output stays in
-// registers. prefix_merge_kernel joins the partial results of both.
+// registers. A call is divided among two CTAs an SM: at D = 64 two fit, at D = 128 (114 KB of shared memory and 1 KB
+// of the system's each, of 228) one does, and the stretches run as two waves. One B200, 8 sequences over 4k keys, 8/2
+// heads of 128, replayed from a graph: one new token each 39 us, 8 each 79 us, 64 each 349 us. prefix_merge_kernel
+// joins the partial results of both.
 
 #include "hc_prefix.cuh"
 

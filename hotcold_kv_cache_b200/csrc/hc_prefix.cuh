@@ -7,8 +7,11 @@
 //   prefix: (KV head, chunk of key tiles, row tile)      suffix: (sequence, KV head, row tile)
 // and all groups lie one behind the other on a line, each as long as it takes (line_cost: so much to start
 // it and so much a key tile). CTA c works on the key tiles that begin in the stretch [c W, (c + 1) W) of the
-// line: whatever the lengths, every CTA gets the same work, and where a stretch ends inside a group its rows
-// are left as several partial results (running maximum, sum, unnormalised output), joined by the merge
+// line, so that CTAs get about the same work: the busiest of 148 has 1.01 times the mean with 64 decode steps over
+// 128k keys and 1.04 with a chunk of 8 x 257 over 16k. Not so where causal own tokens outweigh the rest: every
+// row tile of a sequence is as long on the line as if it saw all of the sequence's keys, and a short last row tile as a
+// whole one (1.29 with 4 x 4096 new tokens over 4k, 1.69 with 8192 over 1k, 1.89 with 16384 and no prefix). Where a
+// stretch ends inside a group its rows are left as several partial results (running maximum, sum, unnormalised output), joined by the merge
 // kernel. A piece (c, group) has its partial rows at  2 * (rows of the groups before it) + c * ROWS:
 // pieces follow one another in c or in the group, and each takes at most min(2 rows, ROWS).
 // The prefix is cut into chunks (nch > 1) when there are several row tiles, so that row tiles reading
@@ -61,9 +64,10 @@ cudaError_t launch_prefix_mma(const PrefixArgs& a, const LineShape& s, int dtype
 // (hc_prefix_mma.cu): above that its halves, below it whole pieces go to one stream each.
 __host__ __device__ inline bool prefix_two_streams(int rows) { return rows > 64 && rows <= 128; }
 
-// fp32: alike. 16 bits, in units of about 0.55 us as measured on whole lines of one kind: tall row tiles
-// 2.8 us a key tile and 4.5 us to load Q and write the result (9.5 us behind causal tiles, where the streams
-// meet and V is looked through), up to 64 rows 1.15 and 1.6 us.
+// fp32: alike. 16 bits, in units of about 0.55 us as measured on whole lines of one kind at D = 128: tall row
+// tiles 2.8 us a key tile and 4.5 us to load Q and write the result (9.5 us behind causal tiles, where the streams
+// meet and V is looked through), up to 64 rows 1.15 and 1.6 us. 65 to 128 rows lie between by choice; a key tile of
+// theirs was measured later at 1.2 us. D = 64 is divided by the same costs: there a key tile takes 2.5 us (tall) and 1.4.
 __device__ __forceinline__ LineCost line_cost(const LineShape& s, int rows, bool own) {
   if (s.dup == 1) return {1, 1};
   if (rows > 128) return {5, own ? 17 : 8};

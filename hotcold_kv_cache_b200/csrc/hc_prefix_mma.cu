@@ -21,10 +21,11 @@
 //
 // Bound: by its bytes up to about 256 rows a row tile, beyond that by the MMAs (1024 cycles per 128 x 128 x 128
 // pair) and the 128 x 128 exponentials (1024 cycles at 16 a cycle) of each tile. Measured on one B200, D = 128
-// in 16 bits: a key tile of 256 rows 2.8 us (its bytes at a 148th of HBM 1.5, MMAs 1.1, exponentials 1.1), of up
-// to 64 rows 1.15 us where pieces alternate; 64 sequences over 128k prefix keys 252 us (2.4 TB/s, 546
-// TFLOP/s), a chunk of 8 x 257 over 16k 440 us (681 TFLOP/s). What the tall tile loses is in its chain: softmax
-// 1.4 us, then [O += P V, next S] 1.4 us, in turns, since P lies over S and the next S has to wait for P V.
+// in 16 bits: a key tile of 256 rows 2.6 to 2.8 us (its bytes at a 148th of HBM 1.5, MMAs 1.1, exponentials 1.1), of
+// 65 to 128 rows 1.2 us, of up to 64 rows 1.15 us where pieces alternate and 1.8 to 3.2 us where a stretch is one
+// piece and so one stream's; 64 sequences over 128k prefix keys 244 us (2.5 TB/s, 564 TFLOP/s), a chunk of 8 x 257
+// over 16k 434 us (690 TFLOP/s). What the tall tile loses is in its chain: softmax 1.4 us, then [O += P V, next S]
+// 1.4 us, in turns, since P lies over S and the next S has to wait for P V.
 
 #include <cuda.h>
 #include <cudaTypedefs.h>

@@ -94,8 +94,8 @@ def plan_pages(lens, new_lens, block_table, free_pages, n_free, page_size: int, 
     the sum of new_lens; rows behind the last token get -1), base_pos the position of a sequence's first
     token (the prefix length). Without `out` the step is committed: lens and n_free are updated in place
     and returned in the plan. With `out`, the plan goes into its tensors; out.lens and out.n_free may be
-    lens and n_free themselves (commit; out.lens may be new_lens too) or others (the step may be thrown away: the next plan starts from
-    the same state). When the tokens do not fit n_tokens, the free pages or the tables, nothing is
+    lens and n_free themselves (commit; out.lens may be new_lens too) or others (the step may be thrown away: the next plan
+    starts from the same state); bits are OR-ed into out.status, which is not cleared. When the tokens do not fit n_tokens, the free pages or the tables, nothing is
     changed, the plan has no tokens and status gets HC_DEV_CAPACITY; a length out of range likewise with
     HC_DEV_INDEX."""
     dev = _cuda("lens", lens)
@@ -228,8 +228,10 @@ def shared_prefix_attention(q, prefix_k, prefix_v, k_pages, v_pages, block_table
     sequence b's n_b attends the prefix keys where prefix_mask (P) bool or uint8 is set (None: all) and
     its own keys j <= lens[b] - n_b + i. Returns out (T,Hq,D), contiguous, and with return_lse the
     natural-log sum of exponentials (T,Hq) float32 too. A row that attends nothing is 0 (lse -inf); rows
-    of no sequence (before cu_new[0], from cu_new[n_seq] on) are left as they were. A table entry outside the pool reads as zero keys and
-    values and sets HC_DEV_INDEX in status (1) int32, when given."""
+    of no sequence (before cu_new[0], from cu_new[n_seq] on) are left as they were. A table entry outside
+    the pool reads as zero keys and values, a length outside the table is cut, and both set HC_DEV_INDEX in
+    status (1) int32, when given. HC_DEV_TIMEOUT there means that a wait inside the kernel ran out and the
+    results are worthless. Without status nothing tells of either."""
     dev = _cuda("q", q)
     if q.dim() != 3:
         raise ValueError(f"q must be (T, Hq, D), not {tuple(q.shape)}")

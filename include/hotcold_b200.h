@@ -388,9 +388,10 @@ HC_API int hc_splice_hits(const hc_layer* L, const int32_t* hit_ids, int k, void
  * running sum of new_lens, and for each of the n_tokens rows t of the step: seq_ids the sequence,
  * slots = page * page_size + row in the page, positions = base_pos + place in the sequence; all three
  * are -1 behind the last token. lens_out / n_free_out may be lens / n_free (the step is committed;
- * lens_out may be new_lens too) or other buffers (it may be thrown away: the next plan writes over it). When the tokens exceed
- * n_tokens, the fresh pages n_free or a sequence max_blocks, or a length is negative or out of range,
- * nothing changes (lens_out = lens, no tokens, slots -1) and status gets HC_DEV_CAPACITY or HC_DEV_INDEX.
+ * lens_out may be new_lens too) or other buffers (it may be thrown away: the next plan writes over it).
+ * When the tokens exceed n_tokens, the fresh pages n_free or a sequence max_blocks, or a length is
+ * negative or out of range, nothing changes (lens_out = lens, no tokens, slots -1) and status gets
+ * HC_DEV_CAPACITY or HC_DEV_INDEX.
  *
  * hc_release_pages: sequence b keeps its first keep_lens[b] <= lens[b] tokens (0 frees it); pages
  * behind them go back on the stack, in the reverse of the order a plan takes them, and lens =
